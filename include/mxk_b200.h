@@ -372,6 +372,72 @@ int mxk_lpt_assign(const int32_t* counts, const int32_t* experts, int n_experts,
 int mxk_gs_schedule_on_device(const int32_t* rows_of_ge, int EPR, int group_ranks, int win_cap, int hot_windows,
                               int32_t* out_ge, int32_t* out_w, int32_t* out_n, int cap);
 
+/* ---- operators beside the layer -------------------------------------------------------------
+ * The layer taken apart: tokens sorted by expert, the experts' products, the rows summed back per
+ * token.  No counterpart in the reference, whose kernel holds these steps inside itself.  All are
+ * asynchronous on the given stream, allocate nothing, keep nothing between calls and can be captured
+ * into a graph; calls on several streams share no workspace.  Pointers are device pointers of the
+ * current device; pair p = token * topk + j. */
+#define MXK_DTYPE_BF16 0
+#define MXK_DTYPE_FP16 1
+#define MXK_DTYPE_FP32 2
+#define MXK_FP8_E4M3 0
+#define MXK_FP8_E5M2 1
+
+/* Rows of the pairs in expert order.  topk_idx [tokens][topk] holds ids of idx_bytes (4 or 8) bytes, idx_stride
+ * ids between tokens; a pair whose id lies outside [first_expert, first_expert + num_experts) is dropped.
+ *   offsets     [num_experts + 1]: expert e's rows are offsets[e] .. offsets[e + 1]
+ *   row_of_pair [tokens * topk]: the pair's row, -1 when dropped; ascending pair index inside an expert
+ *   pair_of_row [tokens * topk]: its inverse, -1 behind offsets[num_experts]
+ * tokens * topk <= 2^30, topk <= 256, num_experts <= 1024. */
+int mxk_plan_tokens(const void* topk_idx, int32_t idx_bytes, int64_t idx_stride, int32_t tokens, int32_t topk,
+                    int32_t first_expert, int32_t num_experts, int32_t* row_of_pair, int32_t* pair_of_row,
+                    int32_t* offsets, void* stream);
+
+/* rows[row_of_pair[p]] = x[p / topk], bytes unchanged (any element type); rows behind offsets[num_experts]
+ * are cleared.  x: tokens rows of row_bytes, x_stride bytes apart; rows: [tokens * topk] rows without gaps.  x_sf
+ * (or NULL): scale bytes that travel with the rows. */
+int mxk_sort_tokens(const void* x, int64_t x_stride, int64_t row_bytes, const void* x_sf, int64_t sf_stride, int64_t sf_bytes,
+                    int32_t tokens, int32_t topk, int32_t num_experts, const int32_t* row_of_pair, const int32_t* offsets,
+                    void* rows, void* rows_sf, void* stream);
+
+/* y[t] = sum over j of weights[t][j] * rows[row_of_pair[t][j]], j ascending, FP32, rounded once to the rows'
+ * type (MXK_DTYPE_*); weights NULL: all one (the gradient of the sort).  Strides: bytes between rows, floats
+ * between the tokens' weights. */
+int mxk_unsort_tokens(const void* rows, int32_t dtype, int64_t rows_stride, const float* weights, int64_t weights_stride,
+                      int32_t tokens, int32_t topk, int32_t hidden, const int32_t* row_of_pair, void* y, void* stream);
+
+/* Gradients of mxk_unsort_tokens with weights: drows[row] = weights * dy of its token (0 behind the last row; NULL:
+ * not wanted), dweights[t][j] = <dy[t], rows[row]> in FP32 (0 for a dropped pair; NULL: not wanted). */
+int mxk_unsort_tokens_grad(const void* dy, int64_t dy_stride, const void* rows, int64_t rows_stride, int32_t dtype,
+                           const float* weights, int64_t weights_stride, int32_t tokens, int32_t topk, int32_t num_experts,
+                           int32_t hidden, const int32_t* row_of_pair, const int32_t* offsets, void* drows, float* dweights,
+                           void* stream);
+
+/* out[m][n] = sum over k of x[m][k] 2^(x_sf[m][k / 128] - 127) * w[n][k] 2^(w_sf - 127), FP32 accumulation, bf16 out.
+ * Dense (offsets NULL), or grouped: rows offsets[e] .. offsets[e + 1] of x and out meet the e-th weight matrix.
+ * Scale planes are UE8M0 exponent bytes (NULL: all one): x_sf [rows][ceil(depth / 128)], x_sf_stride bytes apart;
+ * w_sf per 128 x 128 block [experts][ceil(cols / 128)][ceil(depth / 128)], or per row [experts][cols][...] when
+ * w_sf_per_row (the form of a product whose two factors are both activations, e.g. a weight gradient). */
+typedef struct MxkMatmulArgs {
+    const uint8_t* x;          /* [rows][depth], x_stride bytes between rows (a multiple of 16)   */
+    const uint8_t* x_sf;
+    const uint8_t* w;          /* [experts][cols][depth], w_stride bytes between rows             */
+    const uint8_t* w_sf;
+    uint16_t* out;             /* bf16 [rows][cols], out_stride elements between rows              */
+    const int32_t* offsets;    /* [experts + 1] on the device, or NULL                             */
+    int64_t x_stride, x_sf_stride, w_stride, out_stride;
+    int32_t rows, cols, depth, experts;
+    int32_t x_format, w_format;    /* MXK_FP8_*                                                    */
+    int32_t w_sf_per_row;
+    int32_t zero_tail;         /* grouped: clear out rows of no expert (0: they are left alone)     */
+    int32_t max_spins;         /* bound of every device wait, in units of 250 ns; 0 => 2 s         */
+} MxkMatmulArgs;
+int mxk_fp8_matmul(const MxkMatmulArgs* a, void* stream);
+/* Synchronous: 0, or the MXK_DEV_* code of the first product on this device whose wait expired (its output is
+ * then undefined). */
+int mxk_matmul_status(int32_t* out);
+
 /* Symmetric-memory helpers (reference SymmBuffer C++ side,
  * torch/csrc/apis/mega.hpp:86-195): device allocation that can be exported to
  * the other ranks' processes, and import of their handles. */

@@ -6,6 +6,13 @@ There is no CPU fallback: importing works anywhere, launching needs the built
 library and a B200.
 """
 from . import _lib, quant  # noqa: F401
+from .experts import (  # noqa: F401
+    ExpertPlan,
+    plan_tokens_by_expert,
+    sort_tokens_by_expert,
+    unsort_tokens_by_expert,
+)
+from .matmul import fp8_grouped_matmul, fp8_matmul, matmul_status  # noqa: F401
 from .mega import (  # noqa: F401
     SymmBuffer,
     bf16_fp8_mega_moe,

@@ -18,14 +18,16 @@ NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", 
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile csrc/mxk_kernels.cu for sm_100a into libmxk_b200.so (in-tree)."""
-    srcs = [os.path.join(SRC_DIR, f) for f in ("mxk_kernels.cu", "mxk_device.cuh", "mxk_phases.cuh", "mxk_gemm.cuh",
-                                               "mxk_sched.cuh")]
+    """Compile csrc/mxk_kernels.cu (the layer) and csrc/mxk_operators.cu (the operators beside it) for
+    sm_100a into libmxk_b200.so (in-tree)."""
+    units = [os.path.join(SRC_DIR, f) for f in ("mxk_kernels.cu", "mxk_operators.cu")]
+    srcs = units + [os.path.join(SRC_DIR, f) for f in ("mxk_device.cuh", "mxk_phases.cuh", "mxk_gemm.cuh", "mxk_sched.cuh",
+                                                       "mxk_rows.cuh", "mxk_matmul.cuh")]
     hdr = os.path.join(os.path.dirname(_HERE), "include", "mxk_b200.h")
     newest = max(os.path.getmtime(p) for p in srcs + [hdr])
     if not force and os.path.exists(LIB_PATH) and os.path.getmtime(LIB_PATH) >= newest:
         return LIB_PATH
-    cmd = ["nvcc"] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-o", LIB_PATH, srcs[0]]
+    cmd = ["nvcc"] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["--threads", "2", "-o", LIB_PATH] + units
     subprocess.run(cmd, check=True)
     return LIB_PATH
 
@@ -89,6 +91,7 @@ EXPORTS = [
     "mxk_static_scratch_bytes", "mxk_fill_weights", "mxk_fill_weights_e2m1", "mxk_e2m1_to_e4m3", "mxk_quantize_rows", "mxk_dump_kernel_resources", "mxk_read_status",
     "mxk_read_status_static", "mxk_rwk_ticks_off", "mxk_ticks_count", "mxk_set_ticks", "mxk_select_win",
     "mxk_group_ranks", "mxk_gs_schedule_member", "mxk_gs_schedule_member_hot", "mxk_gs_group_skewed", "mxk_lpt_assign", "mxk_gs_schedule_on_device",
+    "mxk_plan_tokens", "mxk_sort_tokens", "mxk_unsort_tokens", "mxk_unsort_tokens_grad", "mxk_fp8_matmul", "mxk_matmul_status",
     "mxk_symm_alloc", "mxk_symm_free", "mxk_ipc_export", "mxk_ipc_import", "mxk_ipc_close",
 ]
 
@@ -136,6 +139,13 @@ def lib():
     L.mxk_gs_schedule_member_hot.argtypes = [i32p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, i32p, i32p, C.c_int]
     L.mxk_gs_schedule_on_device.argtypes = [i32p, C.c_int, C.c_int, C.c_int, C.c_int, i32p, i32p, i32p, C.c_int]
     L.mxk_select_win.argtypes = [C.POINTER(C.c_uint32), C.c_int, C.c_int, C.c_int]
+    vp, i32, i64 = C.c_void_p, C.c_int32, C.c_int64
+    L.mxk_plan_tokens.argtypes = [vp, i32, i64, i32, i32, i32, i32, vp, vp, vp, vp]
+    L.mxk_sort_tokens.argtypes = [vp, i64, i64, vp, i64, i64, i32, i32, i32, vp, vp, vp, vp, vp]
+    L.mxk_unsort_tokens.argtypes = [vp, i32, i64, vp, i64, i32, i32, i32, vp, vp, vp]
+    L.mxk_unsort_tokens_grad.argtypes = [vp, i64, vp, i64, i32, vp, i64, i32, i32, i32, i32, vp, vp, vp, vp, vp]
+    L.mxk_fp8_matmul.argtypes = [C.c_char_p, vp]     # a packed MxkMatmulArgs
+    L.mxk_matmul_status.argtypes = [C.POINTER(C.c_int32)]
     L.mxk_symm_alloc.argtypes = [C.POINTER(C.c_void_p), C.c_int64]
     L.mxk_symm_free.argtypes = [C.c_void_p]
     L.mxk_ipc_export.argtypes = [C.c_void_p, C.c_char_p]

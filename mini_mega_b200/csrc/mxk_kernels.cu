@@ -742,6 +742,9 @@ int static_scratch_base(uint8_t** out, int* dev_out) {
 
 }  // namespace
 
+// the operators' translation unit reports through the same per-thread message
+__attribute__((visibility("hidden"))) int mxk_set_error(int code, const std::string& msg) { return fail(code, msg); }
+
 // ================================================================== C ABI =====
 extern "C" {
 

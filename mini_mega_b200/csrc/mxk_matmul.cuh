@@ -1,0 +1,506 @@
+// ============================================================================
+// mxk_matmul.cuh — 8-bit products with UE8M0 block scales, apart from the layer.
+//
+//   out[m, n] = sum_k x[m, k] 2^(sx[m, k/128] - 127) * w[n, k] 2^(sw[.., k/128] - 127)
+//
+// dense (one weight matrix) or grouped (rows offsets[e] .. offsets[e+1] of x meet w[e]).
+// The scales are powers of two, one per 128 columns, so the block-scaled tensor-core MMA
+// applies them exactly on its way into one FP32 accumulator over all of K.
+//
+// Orientation: the WEIGHT rows are the M side of the MMA (128 per CTA) and the rows of x its N
+// side, whose extent is a run-time multiple of 16.  An expert with 3 rows then costs an N = 16
+// MMA instead of a 128-row tile, a group of 1100 rows is cut into five equal tiles of 224 instead
+// of nine of 128, and one kernel body serves a single token and a prefill.  The accumulators come out
+// transposed (lane = output column), which the epilogue's stores turn round: the 32 lanes of a
+// warp write 32 neighbouring columns of one output row.
+//
+// A unit of work is a tile of 128 (CTA pair: 256) weight rows x up to bt_max rows of x.  Units
+// are dealt out round-robin; every role walks the same list from the sanitised group table in
+// shared memory, so there is no task queue, no counter in global memory and no workspace: launches
+// on several streams or in several graphs share nothing.
+//
+// Warp roles (384 threads) as in the layer's GEMM phase: warp 0 TMA producer, warp 1 MMA issuer,
+// warps 2-3 scale tiles (global bytes -> shared tile -> tensor memory), warps 4-11 epilogue.  Two
+// accumulators alternate, so the drain of one tile hides under the MMAs of the next.
+//
+// Few tiles (small batches): the K extent is split over the CTAs of a cluster, the partial tiles
+// are exchanged through distributed shared memory and added in the order of the splits, so results
+// do not depend on timing.
+//
+// Every wait is bounded; on expiry the CTA records a status word, unwinds and frees its TMEM.
+// ============================================================================
+#pragma once
+
+constexpr int kMmThreads = 384;
+constexpr int kMmEpiWarps = 8;
+constexpr int kMmFirstEpi = 4;
+constexpr int kMmMaxStages = 12;
+constexpr int kMmMaxSfSlots = 8;
+constexpr int kMmSfTile = 512;                 // 128 rows x 4 scale bytes
+constexpr int kMmSfSlotBytes = 3 * kMmSfTile;  // weight rows, x rows 0-127, x rows 128-255
+constexpr int kMmWBytes = 128 * 128;           // weight tile of one K block
+constexpr int kMmMaxExperts = 1024;
+constexpr int kMmTmemCols = 512;
+constexpr int kMmSmemLimit = 227 * 1024;
+
+struct MmArgs {
+    const uint8_t* x_sf;       // [rows][x_sf_stride] or null (all 127)
+    const uint8_t* w_sf;       // [experts][w_sf_rows][nkb] or null
+    uint16_t* out;             // bf16 [rows][out_stride]
+    const int* offsets;        // [experts + 1] or null (dense)
+    long long x_sf_stride, out_stride;
+    int rows, cols, nkb, experts;
+    int n_tiles;               // weight tiles of a group
+    int bt_max, box;           // rows of x per tile at most; rows per TMA box (pairs: half a tile)
+    int n_stages, sf_slots, acc_stride, sf_col, sf_slot_cols;
+    int splits;                // CTAs (pairs) of a cluster that share a tile's K extent
+    int w_sf_rows, w_per_row;  // rows of a group's weight scale plane; 1: one scale row per weight row
+    int zero_tail;             // clear out rows behind the last group
+    uint32_t formats;          // operand format bits of the instruction descriptor
+    unsigned long long wait_ns;
+};
+
+struct MmSmem {
+    uint64_t full[kMmMaxStages], empty[kMmMaxStages];
+    uint64_t sf_full[kMmMaxSfSlots], sf_empty[kMmMaxSfSlots], sf_peer[kMmMaxSfSlots];
+    uint64_t acc_full[2], acc_empty[2];
+    uint64_t red_full, red_free;     // split-K exchange: all partials written / all partials read
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+struct MmTile {
+    int group, w_row, x_row, bt, valid;   // w_row: first weight row inside the group; x_row: first row of x
+};
+
+// status word of the products on this device: 0, or the first wait that expired
+__device__ int g_mm_status = 0;
+
+// Tile t of the list: groups in order; inside a group the operand with fewer rows turns fastest,
+// so that the other one is read from memory once while the first stays in L2.
+template <bool kPair>
+__device__ __forceinline__ bool mm_tile(const MmArgs& a, const int* start, const int* before, int t, MmTile& o) {
+    if (t >= before[a.experts]) return false;
+    int lo = 0, hi = a.experts;   // last group with before[g] <= t; empty groups share a value with their successor
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (before[mid] <= t) lo = mid; else hi = mid;
+    }
+    const int n = start[lo + 1] - start[lo], tt = (n + a.bt_max - 1) / a.bt_max, i = t - before[lo];
+    const bool rows_fast = n <= a.cols;
+    const int xt = rows_fast ? i % tt : i / a.n_tiles, wt = rows_fast ? i / tt : i % a.n_tiles;
+    o.group = lo;
+    o.bt = (((n + tt - 1) / tt) + 15) & ~15;
+    o.w_row = wt * (kPair ? 256 : 128);
+    o.x_row = start[lo] + xt * o.bt;
+    o.valid = min(o.bt, n - xt * o.bt);
+    return true;
+}
+
+__device__ __forceinline__ void mm_raise(MmSmem* S, int code) {
+    atomicCAS(&g_mm_status, 0, code);
+    *(volatile int*)&S->abort_flag = 1;
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+// commit of a pair's MMAs onto the barrier at this offset in both CTAs of the pair that starts at
+// cluster rank `first` (a signal inside one cluster; no load, no other GPU's memory)
+__device__ __forceinline__ void umma_commit_pair_at(uint32_t bar_smem_addr, uint32_t first) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar_smem_addr), "h"((uint16_t)(3u << first))
+                 : "memory");
+}
+
+template <bool kPair>
+__device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x, const CUtensorMap* tm_w) {
+    extern __shared__ uint8_t mm_smem_raw[];
+    uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(mm_smem_raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t stage_bytes = (uint32_t)kMmWBytes + (uint32_t)a.box * 128u;
+    uint8_t* sf_tiles = tiles + (size_t)a.n_stages * stage_bytes;
+    float* red = reinterpret_cast<float*>(sf_tiles + a.sf_slots * kMmSfSlotBytes);   // [bt_max][128], splits > 1 only
+    MmSmem* S = reinterpret_cast<MmSmem*>(reinterpret_cast<uint8_t*>(red) + (a.splits > 1 ? (size_t)a.bt_max * 512 : 0));
+    int* start = reinterpret_cast<int*>(S + 1);
+    int* before = start + a.experts + 1;  // both [experts + 1]
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t ctas = kPair ? 2u : 1u;
+    const uint32_t crank = (kPair || a.splits > 1) ? cluster_ctarank() : 0u;
+    const uint32_t half = kPair ? (crank & 1u) : 0u;          // which CTA of the pair
+    const uint32_t first = kPair ? (crank & ~1u) : crank;     // cluster rank of the pair's leader
+    const bool leader = half == 0;
+    const int split = (int)(crank / ctas);
+    const bool clustered = kPair || a.splits > 1;
+    volatile int* abort_flag = &S->abort_flag;
+    const uint64_t wait_ns = a.wait_ns;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kMmMaxStages; ++s) { mbar_init(&S->full[s], 1); mbar_init(&S->empty[s], 1); }
+        for (int s = 0; s < kMmMaxSfSlots; ++s) { mbar_init(&S->sf_full[s], 1); mbar_init(&S->sf_empty[s], 1); mbar_init(&S->sf_peer[s], 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&S->acc_full[s], 1); mbar_init(&S->acc_empty[s], kMmEpiWarps * ctas); }
+        mbar_init(&S->red_full, kMmEpiWarps * a.splits);
+        mbar_init(&S->red_free, kMmEpiWarps * a.splits);
+        S->abort_flag = 0;
+        mbar_fence_init();
+        fence_proxy_async_smem();
+        tma_prefetch_desc(tm_x);
+        tma_prefetch_desc(tm_w);
+    }
+    if (warp == 1) {
+        if constexpr (kPair) { tmem_alloc_pair(&S->tmem_base, kMmTmemCols); tmem_relinquish_pair(); }
+        else { tmem_alloc(&S->tmem_base, kMmTmemCols); tmem_relinquish(); }
+    }
+    // Group table.  Offsets come from the device and are not trusted: clamped into [0, rows] and made
+    // ascending (a running maximum), groups are disjoint whatever they held and no tile reaches outside.
+    for (int e = threadIdx.x; e <= a.experts; e += kMmThreads)
+        start[e] = a.offsets ? min(max(a.offsets[e], 0), a.rows) : e * a.rows;
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {   // running maximum of the offsets, then the exclusive sum of the groups' tile counts
+        int run = 0;
+        for (int e0 = 0; e0 <= a.experts; e0 += 32) {
+            const int e = e0 + lane;
+            int m = e <= a.experts ? start[e] : 0;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) m = max(m, __shfl_up_sync(0xFFFFFFFFu, m, d));   // lanes below d get their own value
+            m = max(m, run);
+            if (e <= a.experts) start[e] = m;
+            run = __shfl_sync(0xFFFFFFFFu, m, 31);
+        }
+        __syncwarp();
+        run = 0;
+        for (int e0 = 0; e0 < a.experts; e0 += 32) {
+            const int e = e0 + lane;
+            const int v = e < a.experts ? ((start[e + 1] - start[e] + a.bt_max - 1) / a.bt_max) * a.n_tiles : 0;
+            int s = v;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xFFFFFFFFu, s, d);
+                if (lane >= d) s += o;
+            }
+            if (e < a.experts) before[e] = run + s - v;
+            run += __shfl_sync(0xFFFFFFFFu, s, 31);
+        }
+        if (lane == 0) before[a.experts] = run;
+    }
+    if (clustered) cluster_sync_all(); else __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *(volatile uint32_t*)&S->tmem_base;
+
+    const int unit = (int)blockIdx.x / (int)(ctas * a.splits), n_units = (int)gridDim.x / (int)(ctas * a.splits);
+    // K blocks of this split, cut at multiples of four blocks (one scale word holds four)
+    const int groups_all = (a.nkb + 3) >> 2;
+    const int g_first = groups_all * split / a.splits, g_last = groups_all * (split + 1) / a.splits;
+    const int kb_first = g_first * 4, kb_last = min(a.nkb, g_last * 4);
+
+    auto wait_bar = [&](uint64_t* bar, uint32_t parity) -> bool {
+        if constexpr (kPair) return mbar_wait_cluster(bar, parity, wait_ns, abort_flag);
+        else return mbar_wait(bar, parity, wait_ns, abort_flag);
+    };
+    auto arrive_leader = [&](uint64_t* bar) {
+        if constexpr (kPair) mbar_arrive_cluster(mapa_u32(smem_u32(bar), first));
+        else mbar_arrive(bar);
+    };
+    MmTile tl;
+
+    if (warp == 0) {
+        // --------------------------------------------------------------- TMA producer
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            unsigned long long issued = 0;
+            bool dead = false;
+            const uint32_t tx = ctas * stage_bytes;
+            for (int t = unit; !dead && mm_tile<kPair>(a, start, before, t, tl); t += n_units) {
+                // rows of all experts lie behind one another in the weight map; a tile that runs past its
+                // expert's last row reads the next expert's, and those output columns are not stored
+                const int w_row = (int)((long long)tl.group * a.cols) + tl.w_row + 128 * (int)half;
+                const int x_row = tl.x_row + (kPair ? (int)half * (tl.bt >> 1) : 0);
+                for (int kb = kb_first; kb < kb_last; ++kb) {
+                    if (!mbar_wait(&S->empty[stage], phase ^ 1, wait_ns, abort_flag)) { dead = true; break; }
+                    uint8_t* sw = tiles + (size_t)stage * stage_bytes;
+                    if constexpr (kPair) {
+                        if (leader) mbar_expect_tx(&S->full[stage], tx);
+                        const uint32_t bar = mapa_u32(smem_u32(&S->full[stage]), first);
+                        tma_load_2d_pair(sw, tm_w, kb * 128, w_row, bar);
+                        tma_load_2d_pair(sw + kMmWBytes, tm_x, kb * 128, x_row, bar);
+                    } else {
+                        mbar_expect_tx(&S->full[stage], tx);
+                        tma_load_2d(sw, tm_w, kb * 128, w_row, &S->full[stage]);
+                        tma_load_2d(sw + kMmWBytes, tm_x, kb * 128, x_row, &S->full[stage]);
+                    }
+                    ++issued;
+                    if (++stage == (uint32_t)a.n_stages) { stage = 0; phase ^= 1; }
+                }
+            }
+            if (dead || *abort_flag) {
+                if (dead) mm_raise(S, MXK_DEV_TIMEOUT_PIPE);
+                // nothing may still be on its way into this shared memory when the CTA ends
+                const unsigned long long n = issued < (unsigned long long)a.n_stages ? issued : (unsigned long long)a.n_stages;
+                for (unsigned long long i = issued - n; leader && i < issued; ++i)
+                    (void)mbar_wait(&S->full[i % a.n_stages], (uint32_t)((i / a.n_stages) & 1), 100000000ull, nullptr);
+            }
+        }
+    } else if (warp == 1) {
+        // ----------------------------------------------------------------- MMA issuer
+        if (lane == 0 && leader) {
+            uint32_t stage = 0, phase = 0, sfg = 0, it = 0;
+            bool stage_ready = false, dead = false;
+            const uint64_t desc0 = umma_smem_desc_sw128(smem_u32(tiles));
+            const uint32_t desc_step = stage_bytes >> 4;
+            for (int t = unit; !dead && mm_tile<kPair>(a, start, before, t, tl); t += n_units, ++it) {
+                const uint32_t buf = it & 1u, use = it >> 1;
+                if (!wait_bar(&S->acc_empty[buf], (use & 1u) ^ 1u)) { dead = true; break; }
+                const uint32_t idesc0 = umma_idesc_mx_e4m3(kPair ? 256 : 128, tl.bt, 0, 0) | a.formats;
+                const uint32_t tacc = tmem_base + buf * (uint32_t)a.acc_stride;
+                uint32_t acc = 0;
+                for (int kb0 = kb_first; kb0 < kb_last && !dead; kb0 += 4) {
+                    const uint32_t slot = sfg % (uint32_t)a.sf_slots;
+                    if (!wait_bar(&S->sf_full[slot], (sfg / (uint32_t)a.sf_slots) & 1u)) { dead = true; break; }
+                    const uint32_t tsf = tmem_base + (uint32_t)a.sf_col + slot * (uint32_t)a.sf_slot_cols;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (kb0 + i >= kb_last) break;
+                        if (!stage_ready && !wait_bar(&S->full[stage], phase)) { dead = true; break; }
+                        tc_fence_after();
+                        const uint64_t wdesc = desc0 + (uint64_t)(stage * desc_step);
+                        const uint64_t xdesc = wdesc + (uint64_t)(kMmWBytes >> 4);
+                        const uint32_t idesc = idesc0 | ((uint32_t)i << 4) | ((uint32_t)i << 29);   // scale byte i of the group
+                        uint32_t nstage = stage + 1, nphase = phase;
+                        if (nstage == (uint32_t)a.n_stages) { nstage = 0; nphase ^= 1; }
+                        if constexpr (kPair) {
+                            umma_mxf8_pair(tacc, wdesc, xdesc, idesc, tsf, tsf + 4, acc);
+                            umma_mxf8_pair(tacc, wdesc + 2, xdesc + 2, idesc, tsf, tsf + 4, 1u);
+                            stage_ready = mbar_try_wait_cluster(&S->full[nstage], nphase);   // polled under the MMAs already queued
+                            umma_mxf8_pair(tacc, wdesc + 4, xdesc + 4, idesc, tsf, tsf + 4, 1u);
+                            umma_mxf8_pair(tacc, wdesc + 6, xdesc + 6, idesc, tsf, tsf + 4, 1u);
+                            umma_commit_pair_at(smem_u32(&S->empty[stage]), first);
+                        } else {
+                            umma_mxf8(tacc, wdesc, xdesc, idesc, tsf, tsf + 4, acc);
+                            umma_mxf8(tacc, wdesc + 2, xdesc + 2, idesc, tsf, tsf + 4, 1u);
+                            stage_ready = mbar_try_wait(&S->full[nstage], nphase);
+                            umma_mxf8(tacc, wdesc + 4, xdesc + 4, idesc, tsf, tsf + 4, 1u);
+                            umma_mxf8(tacc, wdesc + 6, xdesc + 6, idesc, tsf, tsf + 4, 1u);
+                            umma_commit(&S->empty[stage]);
+                        }
+                        acc = 1u;
+                        stage = nstage; phase = nphase;
+                    }
+                    if (dead) break;
+                    if constexpr (kPair) umma_commit_pair_at(smem_u32(&S->sf_empty[slot]), first);
+                    else umma_commit(&S->sf_empty[slot]);
+                    ++sfg;
+                }
+                if (dead) break;
+                if constexpr (kPair) umma_commit_pair_at(smem_u32(&S->acc_full[buf]), first);
+                else umma_commit(&S->acc_full[buf]);
+            }
+            if (dead) mm_raise(S, MXK_DEV_TIMEOUT_PIPE);
+        }
+    } else if (warp == 2 || warp == 3) {
+        // -------------------------------------------------------- scale-tile builders
+        // The two warps take the groups of four K blocks in turn.  Tile byte 16*l + 4*j + i is the
+        // scale of row l + 32*j for K block i of the group (what tcgen05.cp 32x128b.warpx4 wants).
+        const uint32_t mine = (uint32_t)(warp - 2);
+        const bool x_words = a.x_sf && ((a.x_sf_stride | (long long)(reinterpret_cast<uintptr_t>(a.x_sf))) & 3) == 0;
+        const bool w_words = a.w_sf && ((a.nkb | (int)(reinterpret_cast<uintptr_t>(a.w_sf) & 3)) & 3) == 0;
+        auto load_word = [&](const uint8_t* p, int kb, bool words) -> uint32_t {   // p: the row's first scale byte
+            if (words && kb + 4 <= a.nkb) return __ldg(reinterpret_cast<const uint32_t*>(p + kb));
+            uint32_t v = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v |= (kb + i < a.nkb ? (uint32_t)__ldg(p + kb + i) : 127u) << (8 * i);
+            return v;
+        };
+        constexpr int kXj = kPair ? 8 : 4;
+        uint32_t sfg = 0;
+        bool dead = false;
+        for (int t = unit; !dead && mm_tile<kPair>(a, start, before, t, tl); t += n_units) {
+            const uint8_t* wsf = nullptr;
+            int w_here = 0;   // weight rows of this CTA's half that exist
+            if (a.w_sf) {
+                const int r0 = tl.w_row + 128 * (int)half;
+                w_here = a.cols - r0;
+                const long long plane = (long long)tl.group * a.w_sf_rows;
+                wsf = a.w_sf + (plane + (a.w_per_row ? r0 : r0 >> 7)) * a.nkb;
+            }
+            const uint8_t* xsf = a.x_sf ? a.x_sf + (long long)tl.x_row * a.x_sf_stride : nullptr;
+            auto load_group = [&](int g, uint32_t (&wx)[kXj], uint32_t (&ww)[4]) {
+                const int kb = g * 4;
+#pragma unroll
+                for (int j = 0; j < kXj; ++j) {
+                    const int r = lane + 32 * j;
+                    wx[j] = (xsf && r < tl.valid) ? load_word(xsf + (long long)r * a.x_sf_stride, kb, x_words) : 0x7F7F7F7Fu;
+                }
+                if (!a.w_per_row) {   // a 128 x 128 block: one word for all rows
+                    const uint32_t v = (wsf && w_here > 0) ? load_word(wsf, kb, w_words) : 0x7F7F7F7Fu;
+                    ww[0] = ww[1] = ww[2] = ww[3] = v;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = lane + 32 * j;
+                        ww[j] = (wsf && r < w_here) ? load_word(wsf + (long long)r * a.nkb, kb, w_words) : 0x7F7F7F7Fu;
+                    }
+                }
+            };
+            const int n_groups = g_last - g_first;
+            int i0 = (int)((mine ^ sfg) & 1u);    // first group of this tile that is this warp's
+            uint32_t wx[kXj], ww[4];
+            if (i0 < n_groups) load_group(g_first + i0, wx, ww);
+            for (int i = i0; i < n_groups; i += 2) {
+                const uint32_t gg = sfg + (uint32_t)i, slot = gg % (uint32_t)a.sf_slots, par = (gg / (uint32_t)a.sf_slots) & 1u;
+                bool ok = true;
+                if (lane == 0) ok = wait_bar(&S->sf_empty[slot], par ^ 1u);
+                ok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;
+                if (!ok) { dead = true; break; }
+                uint4* dst = reinterpret_cast<uint4*>(sf_tiles + slot * kMmSfSlotBytes);
+                dst[lane] = make_uint4(ww[0], ww[1], ww[2], ww[3]);
+                dst[32 + lane] = make_uint4(wx[0], wx[1], wx[2], wx[3]);
+                if constexpr (kPair) dst[64 + lane] = make_uint4(wx[4], wx[5], wx[6], wx[7]);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (i + 2 < n_groups) load_group(g_first + i + 2, wx, ww);   // in flight while the copy is issued and the slot awaited
+                if (lane == 0) {
+                    const uint32_t tsf = tmem_base + (uint32_t)a.sf_col + slot * (uint32_t)a.sf_slot_cols;
+                    const uint64_t sfdesc = umma_smem_desc_sf(smem_u32(dst));
+                    if constexpr (kPair) {
+                        if (leader) {   // one copy serves both CTAs: the partner's tile must be in place
+                            ok = wait_bar(&S->sf_peer[slot], par);
+                            if (ok) {
+                                tc_fence_after();
+                                utccp_32x128b_warpx4_pair(tsf, sfdesc);
+                                utccp_32x128b_warpx4_pair(tsf + 4, sfdesc + (kMmSfTile >> 4));
+                                utccp_32x128b_warpx4_pair(tsf + 8, sfdesc + (2 * kMmSfTile >> 4));
+                                umma_commit_pair(mapa_u32(smem_u32(&S->sf_full[slot]), first));
+                            }
+                        } else {
+                            arrive_leader(&S->sf_peer[slot]);
+                        }
+                    } else {
+                        tc_fence_after();
+                        utccp_32x128b_warpx4(tsf, sfdesc);
+                        utccp_32x128b_warpx4(tsf + 4, sfdesc + (kMmSfTile >> 4));
+                        umma_commit(&S->sf_full[slot]);
+                    }
+                }
+                ok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;
+                if (!ok) { dead = true; break; }
+            }
+            sfg += (uint32_t)n_groups;
+        }
+        if (dead && lane == 0) mm_raise(S, MXK_DEV_TIMEOUT_PIPE);
+    } else {
+        // ------------------------------------------------------------------- epilogue
+        // Warp (q, part) reads TMEM lanes 32q .. 32q+31 (its output columns) and every second chunk of
+        // 16 accumulator columns (rows of x).
+        const int q = warp & 3, part = (warp - kMmFirstEpi) >> 2;
+        uint32_t it = 0;
+        bool dead = false;
+        for (int t = unit; mm_tile<kPair>(a, start, before, t, tl); t += n_units, ++it) {
+            const uint32_t buf = it & 1u, use = it >> 1;
+            bool ok = true;
+            if (lane == 0) ok = wait_bar(&S->acc_full[buf], use & 1u);
+            ok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;
+            // the previous tile's partials have been read by every split before they are overwritten
+            if (ok && a.splits > 1 && it > 0) ok = mbar_wait_cluster(&S->red_free, (it - 1) & 1u, wait_ns, abort_flag);
+            ok = __all_sync(0xFFFFFFFFu, ok ? 1 : 0) != 0;
+            if (!ok) { dead = true; break; }
+            tc_fence_after();
+            const uint32_t tacc = tmem_base + buf * (uint32_t)a.acc_stride + ((uint32_t)(q * 32) << 16);
+            const int n_chunks = tl.bt >> 4;
+            const int col = tl.w_row + 128 * (int)half + q * 32 + lane;
+            const bool col_ok = col < a.cols;
+            uint16_t* out = a.out + (long long)tl.x_row * a.out_stride + col;
+            for (int c = part; c < n_chunks; c += 4) {
+                uint32_t v[2][16];
+                const bool two = c + 2 < n_chunks;
+                tmem_ld16(tacc + c * 16, v[0]);
+                if (two) tmem_ld16(tacc + (c + 2) * 16, v[1]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    if (u == 1 && !two) break;
+                    const int r0 = (c + 2 * u) * 16;
+                    if (a.splits > 1) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) red[(r0 + j) * 128 + q * 32 + lane] = __uint_as_float(v[u][j]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (col_ok && r0 + j < tl.valid)
+                                out[(long long)(r0 + j) * a.out_stride] = __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(v[u][j])));
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_leader(&S->acc_empty[buf]);
+            if (a.splits > 1) {
+                // every split's partial tile is in its own shared memory; split s adds up rows s, s + splits, ...
+                const uint32_t peer_step = ctas;
+                if (lane == 0)
+                    for (int s = 0; s < a.splits; ++s) mbar_arrive_cluster(mapa_u32(smem_u32(&S->red_full), (uint32_t)s * peer_step + half));
+                ok = mbar_wait_cluster(&S->red_full, it & 1u, wait_ns, abort_flag);
+                ok = __all_sync(0xFFFFFFFFu, ok ? 1 : 0) != 0;
+                if (!ok) { dead = true; break; }
+                const int c0 = tl.w_row + 128 * (int)half + lane * 4;
+                for (int r = split + a.splits * (warp - kMmFirstEpi); r < tl.valid; r += a.splits * kMmEpiWarps) {
+                    const uint32_t at = smem_u32(red + r * 128 + lane * 4);
+                    float4 sum = ld_cluster_f4(mapa_u32(at, half));
+                    for (int s = 1; s < a.splits; ++s) {
+                        const float4 o = ld_cluster_f4(mapa_u32(at, (uint32_t)s * peer_step + half));
+                        sum.x += o.x; sum.y += o.y; sum.z += o.z; sum.w += o.w;
+                    }
+                    uint16_t* dst = a.out + (long long)(tl.x_row + r) * a.out_stride + c0;
+                    const uint32_t lo = pack_bf16x2(sum.x, sum.y), hi = pack_bf16x2(sum.z, sum.w);
+                    if (c0 + 4 <= a.cols && (reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
+                        *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+                    } else {
+                        if (c0 < a.cols) dst[0] = (uint16_t)lo;
+                        if (c0 + 1 < a.cols) dst[1] = (uint16_t)(lo >> 16);
+                        if (c0 + 2 < a.cols) dst[2] = (uint16_t)hi;
+                        if (c0 + 3 < a.cols) dst[3] = (uint16_t)(hi >> 16);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0)
+                    for (int s = 0; s < a.splits; ++s) mbar_arrive_cluster(mapa_u32(smem_u32(&S->red_free), (uint32_t)s * peer_step + half));
+            }
+        }
+        if (dead && lane == 0) mm_raise(S, MXK_DEV_TIMEOUT_PIPE);
+        if (a.zero_tail) {   // rows of no group: out was allocated for them, nothing computes them
+            const int head = start[0], end = start[a.experts], n = head + a.rows - end;
+            const int tid = (int)threadIdx.x - kMmFirstEpi * 32;
+            for (int i = (int)blockIdx.x; i < n; i += (int)gridDim.x) {
+                const long long r = i < head ? i : (long long)end + (i - head);
+                for (int c = tid; c < a.cols; c += kMmEpiWarps * 32) a.out[r * a.out_stride + c] = 0;
+            }
+        }
+    }
+    // nobody leaves while the partner may still signal or read this CTA's shared memory
+    tc_fence_before();
+    if (clustered) cluster_sync_all(); else __syncthreads();
+    tc_fence_after();
+    if (warp == 1) {
+        if constexpr (kPair) tmem_dealloc_pair(tmem_base, kMmTmemCols); else tmem_dealloc(tmem_base, kMmTmemCols);
+    }
+}
+
+__global__ void __launch_bounds__(kMmThreads, 1)
+k_matmul(const MmArgs a, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w) {
+    mm_body<false>(a, &tm_x, &tm_w);
+}
+__global__ void __launch_bounds__(kMmThreads, 1)
+k_matmul_pair(const MmArgs a, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w) {
+    mm_body<true>(a, &tm_x, &tm_w);
+}

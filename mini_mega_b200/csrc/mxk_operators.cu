@@ -1,0 +1,338 @@
+// ============================================================================
+// mxk_operators.cu — operators beside the layer, behind the C ABI of include/mxk_b200.h: tokens
+// sorted by expert and back with their gradients (mxk_rows.cuh), 8-bit products with block scales,
+// dense and grouped by expert (mxk_matmul.cuh).
+// ============================================================================
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cstring>
+#include <string>
+
+#include "../../include/mxk_b200.h"
+#include "mxk_device.cuh"
+
+// mxk_last_error()'s message of this thread (mxk_kernels.cu)
+__attribute__((visibility("hidden"))) int mxk_set_error(int code, const std::string& msg);
+
+namespace {
+
+using namespace mxk;
+
+#include "mxk_rows.cuh"
+#include "mxk_matmul.cuh"
+
+constexpr int kSms = 148;
+
+int fail(int code, const std::string& msg) { return mxk_set_error(code, msg); }
+int cuda_fail(cudaError_t e, const char* what) { return mxk_set_error((int)e, std::string(what) + ": " + cudaGetErrorString(e)); }
+int launched(const char* what) {
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? 0 : cuda_fail(e, what);
+}
+
+// Largest power of two up to 16 that divides every given address, stride and length (in bytes).
+int common_vec(uint64_t bits) {
+    bits |= 16;
+    return (int)(bits & (~bits + 1));
+}
+uint64_t addr(const void* p) { return (uint64_t)reinterpret_cast<uintptr_t>(p); }
+
+// Dynamic shared memory above 48 KB has to be allowed once per kernel and device.
+int allow_smem(const void* fn, int slot, int bytes) {
+    static thread_local uint64_t done[3] = {0, 0, 0};   // bit = device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+    if (dev < 64 && (done[slot] >> dev) & 1) return 0;
+    int major = 0;
+    if ((e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev)) != cudaSuccess) return cuda_fail(e, "cudaDeviceGetAttribute");
+    if (major != 10) return fail(MXK_ERR_DEVICE, "the operators run on sm_100 devices only");
+    if ((e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
+    if (dev < 64) done[slot] |= 1ull << dev;
+    return 0;
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+    static const EncodeTiledFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) p = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(p);
+    }();
+    return fn;
+}
+// bytes [rows][k] with `stride` bytes between rows, tiles of box_rows x 128 bytes, 128-byte swizzle, zero outside
+int byte_map(CUtensorMap* m, const void* base, int64_t rows, int64_t k, int64_t stride, int box_rows) {
+    const EncodeTiledFn enc = encode_fn();
+    if (!enc) return fail(MXK_ERR_NO_DRIVER, "cuTensorMapEncodeTiled not available from the CUDA driver");
+    const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : fail(MXK_ERR_TENSOR_MAP, "cuTensorMapEncodeTiled failed, CUresult " + std::to_string((int)r));
+}
+
+// Work split of the row kernels: `span` whole rows per CTA of narrow rows, column parts of one row
+// when rows are wide or few.
+struct RowGrid { int span, vecs, part_vecs, threads; dim3 grid; };
+RowGrid row_grid(int tokens, int row_bytes, int vec) {
+    RowGrid g;
+    g.vecs = row_bytes / vec;
+    g.span = std::max(1, 512 / g.vecs);
+    g.part_vecs = g.vecs;
+    if (g.span == 1) {
+        const int parts_min = (g.vecs + 1023) / 1024;
+        const int parts_fill = std::min((g.vecs + 63) / 64, (2 * kSms + tokens - 1) / tokens);   // few tokens: more CTAs per row
+        const int parts = std::min(65535, std::max(parts_min, parts_fill));
+        g.part_vecs = (g.vecs + parts - 1) / parts;
+    } else {
+        g.span = std::max(1, std::min(g.span, (tokens + 2 * kSms - 1) / (2 * kSms)));
+    }
+    const int work = g.span * g.part_vecs;
+    g.threads = std::min(256, std::max(64, (work + 31) / 32 * 32));
+    g.grid = dim3((unsigned)((tokens + g.span - 1) / g.span), (unsigned)((g.vecs + g.part_vecs - 1) / g.part_vecs), 1);
+    return g;
+}
+
+int bad_tables(int64_t tokens, int topk) { return tokens < 0 || topk < 1 || topk > 256 || tokens * topk > (1 << 30); }
+
+template <int kType>
+int unsort_launch(const UnsortArgs& a, int vec, const RowGrid& g, cudaStream_t st) {
+    switch (vec) {
+        case 16: k_unsort_rows<kType, 16><<<g.grid, g.threads, 0, st>>>(a); break;
+        case 8: k_unsort_rows<kType, 8><<<g.grid, g.threads, 0, st>>>(a); break;
+        case 4: k_unsort_rows<kType, 4><<<g.grid, g.threads, 0, st>>>(a); break;
+        default:
+            if constexpr (kType != kTypeFp32) k_unsort_rows<kType, 2><<<g.grid, g.threads, 0, st>>>(a);
+    }
+    return launched("launch k_unsort_rows");
+}
+template <int kType>
+int unsort_grad_launch(const UnsortGradArgs& a, int vec, int grid, int threads, cudaStream_t st) {
+    switch (vec) {
+        case 16: k_unsort_grad<kType, 16><<<grid, threads, 0, st>>>(a); break;
+        case 8: k_unsort_grad<kType, 8><<<grid, threads, 0, st>>>(a); break;
+        case 4: k_unsort_grad<kType, 4><<<grid, threads, 0, st>>>(a); break;
+        default:
+            if constexpr (kType != kTypeFp32) k_unsort_grad<kType, 2><<<grid, threads, 0, st>>>(a);
+    }
+    return launched("launch k_unsort_grad");
+}
+
+int dtype_bytes(int dtype) { return dtype == MXK_DTYPE_FP32 ? 4 : 2; }
+
+}  // namespace
+
+extern "C" {
+
+int mxk_plan_tokens(const void* topk_idx, int32_t idx_bytes, int64_t idx_stride, int32_t tokens, int32_t topk,
+                    int32_t first_expert, int32_t num_experts, int32_t* row_of_pair, int32_t* pair_of_row,
+                    int32_t* offsets, void* stream) {
+    if (bad_tables(tokens, topk) || num_experts < 1 || num_experts > kRowsMaxExperts || first_expert < 0 || (idx_bytes != 4 && idx_bytes != 8))
+        return fail(MXK_ERR_BAD_ARG, "plan_tokens: need tokens * topk <= 2^30, 1 <= topk <= 256, 1 <= num_experts <= 1024, ids of 4 or 8 bytes");
+    if (!offsets || (tokens > 0 && (!topk_idx || !row_of_pair || !pair_of_row)))
+        return fail(MXK_ERR_BAD_ARG, "plan_tokens: pointers must be non-null");
+    PlanArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.idx = topk_idx; a.idx_stride = idx_stride; a.idx64 = idx_bytes == 8;
+    a.pairs = tokens * topk; a.topk = topk; a.first = first_expert; a.experts = num_experts;
+    a.ftopk = FastDiv::make((uint32_t)topk);
+    a.row_of_pair = row_of_pair; a.pair_of_row = pair_of_row; a.offsets = offsets;
+    const int ctas = a.pairs > kPlanThreads * kPlanKeep ? kPlanClusterMax : 1;
+    a.per_warp = ((a.pairs + ctas * kPlanWarps - 1) / (ctas * kPlanWarps) + 31) / 32 * 32;
+    if (a.per_warp == 0) a.per_warp = 32;
+    a.per_cta = a.per_warp * kPlanWarps;
+    if (int rc = allow_smem((const void*)k_plan, 0, (kPlanWarps + 1) * kRowsMaxExperts * 4)) return rc;
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(ctas, 1, 1); cfg.blockDim = dim3(kPlanThreads, 1, 1);
+    cfg.dynamicSmemBytes = (size_t)(kPlanWarps + 1) * num_experts * 4;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = ctas; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+    cfg.attrs = &at; cfg.numAttrs = ctas > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, k_plan, a);
+    return e == cudaSuccess ? 0 : cuda_fail(e, "launch k_plan");
+}
+
+int mxk_sort_tokens(const void* x, int64_t x_stride, int64_t row_bytes, const void* x_sf, int64_t sf_stride, int64_t sf_bytes,
+                    int32_t tokens, int32_t topk, int32_t num_experts, const int32_t* row_of_pair, const int32_t* offsets,
+                    void* rows, void* rows_sf, void* stream) {
+    if (bad_tables(tokens, topk) || num_experts < 1 || num_experts > kRowsMaxExperts || row_bytes < 1 || row_bytes > (1 << 28) || (x_sf && (sf_bytes < 1 || sf_bytes > (1 << 24))))
+        return fail(MXK_ERR_BAD_ARG, "sort_tokens: sizes out of range");
+    if (tokens == 0) return 0;
+    if (!x || !rows || !row_of_pair || !offsets || (x_sf && !rows_sf)) return fail(MXK_ERR_BAD_ARG, "sort_tokens: pointers must be non-null");
+    const int vec = common_vec(addr(x) | addr(rows) | (uint64_t)x_stride | (uint64_t)row_bytes);
+    SortArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.x = static_cast<const uint8_t*>(x); a.x_sf = static_cast<const uint8_t*>(x_sf);
+    a.rows = static_cast<uint8_t*>(rows); a.rows_sf = static_cast<uint8_t*>(rows_sf);
+    a.row_of_pair = row_of_pair; a.end = offsets + num_experts;
+    a.x_stride = x_stride; a.sf_stride = sf_stride; a.row_bytes = (int)row_bytes; a.sf_bytes = (int)sf_bytes;
+    if (x_sf) {
+        const int v = common_vec(addr(x_sf) | addr(rows_sf) | (uint64_t)sf_stride | (uint64_t)sf_bytes);
+        a.sf_vec = v == 2 ? 1 : v;
+    }
+    const RowGrid g = row_grid(tokens, a.row_bytes, vec);
+    a.tokens = tokens; a.topk = topk; a.pairs = tokens * topk; a.span = g.span; a.vecs = g.vecs; a.part_vecs = g.part_vecs;
+    a.fvecs = FastDiv::make((uint32_t)g.vecs);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    switch (vec) {
+        case 16: k_sort_rows<16><<<g.grid, g.threads, 0, st>>>(a); break;
+        case 8: k_sort_rows<8><<<g.grid, g.threads, 0, st>>>(a); break;
+        case 4: k_sort_rows<4><<<g.grid, g.threads, 0, st>>>(a); break;
+        case 2: k_sort_rows<2><<<g.grid, g.threads, 0, st>>>(a); break;
+        default: k_sort_rows<1><<<g.grid, g.threads, 0, st>>>(a); break;
+    }
+    return launched("launch k_sort_rows");
+}
+
+int mxk_unsort_tokens(const void* rows, int32_t dtype, int64_t rows_stride, const float* weights, int64_t weights_stride,
+                      int32_t tokens, int32_t topk, int32_t hidden, const int32_t* row_of_pair, void* y, void* stream) {
+    if (bad_tables(tokens, topk) || hidden < 1 || hidden > (1 << 26) || dtype < MXK_DTYPE_BF16 || dtype > MXK_DTYPE_FP32)
+        return fail(MXK_ERR_BAD_ARG, "unsort_tokens: sizes or type out of range");
+    if (tokens == 0) return 0;
+    if (!rows || !row_of_pair || !y) return fail(MXK_ERR_BAD_ARG, "unsort_tokens: pointers must be non-null");
+    UnsortArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.rows = static_cast<const uint8_t*>(rows); a.w = weights; a.y = static_cast<uint8_t*>(y); a.row_of_pair = row_of_pair;
+    a.rows_stride = rows_stride; a.w_stride = weights_stride; a.row_bytes = hidden * dtype_bytes(dtype);
+    const int vec = common_vec(addr(rows) | addr(y) | (uint64_t)rows_stride | (uint64_t)a.row_bytes);
+    if (vec < dtype_bytes(dtype)) return fail(MXK_ERR_BAD_ARG, "unsort_tokens: rows and y must be aligned to their element type");
+    const RowGrid g = row_grid(tokens, a.row_bytes, vec);
+    a.tokens = tokens; a.topk = topk; a.pairs = tokens * topk; a.span = g.span; a.vecs = g.vecs; a.part_vecs = g.part_vecs;
+    a.fvecs = FastDiv::make((uint32_t)g.vecs);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == MXK_DTYPE_BF16) return unsort_launch<kTypeBf16>(a, vec, g, st);
+    if (dtype == MXK_DTYPE_FP16) return unsort_launch<kTypeFp16>(a, vec, g, st);
+    return unsort_launch<kTypeFp32>(a, vec, g, st);
+}
+
+int mxk_unsort_tokens_grad(const void* dy, int64_t dy_stride, const void* rows, int64_t rows_stride, int32_t dtype,
+                           const float* weights, int64_t weights_stride, int32_t tokens, int32_t topk, int32_t num_experts,
+                           int32_t hidden, const int32_t* row_of_pair, const int32_t* offsets, void* drows, float* dweights,
+                           void* stream) {
+    if (bad_tables(tokens, topk) || num_experts < 1 || num_experts > kRowsMaxExperts || hidden < 1 || hidden > (1 << 26) || dtype < MXK_DTYPE_BF16 || dtype > MXK_DTYPE_FP32)
+        return fail(MXK_ERR_BAD_ARG, "unsort_tokens_grad: sizes or type out of range");
+    if (tokens == 0 || (!drows && !dweights)) return 0;
+    if (!dy || !weights || !row_of_pair || !offsets || (dweights && !rows)) return fail(MXK_ERR_BAD_ARG, "unsort_tokens_grad: pointers must be non-null");
+    UnsortGradArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.dy = static_cast<const uint8_t*>(dy); a.rows = static_cast<const uint8_t*>(rows); a.w = weights;
+    a.drows = static_cast<uint8_t*>(drows); a.dw = dweights; a.row_of_pair = row_of_pair; a.end = offsets + num_experts;
+    a.dy_stride = dy_stride; a.rows_stride = rows_stride; a.w_stride = weights_stride;
+    a.row_bytes = hidden * dtype_bytes(dtype); a.tokens = tokens; a.topk = topk; a.pairs = tokens * topk;
+    uint64_t bits = addr(dy) | (uint64_t)dy_stride | (uint64_t)a.row_bytes;
+    if (drows) bits |= addr(drows);
+    if (dweights) bits |= addr(rows) | (uint64_t)rows_stride;
+    const int vec = common_vec(bits);
+    if (vec < dtype_bytes(dtype)) return fail(MXK_ERR_BAD_ARG, "unsort_tokens_grad: tensors must be aligned to their element type");
+    a.vecs = a.row_bytes / vec;
+    const int threads = std::min(256, std::max(32, (a.vecs + 31) / 32 * 32));
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == MXK_DTYPE_BF16) return unsort_grad_launch<kTypeBf16>(a, vec, tokens, threads, st);
+    if (dtype == MXK_DTYPE_FP16) return unsort_grad_launch<kTypeFp16>(a, vec, tokens, threads, st);
+    return unsort_grad_launch<kTypeFp32>(a, vec, tokens, threads, st);
+}
+
+int mxk_fp8_matmul(const MxkMatmulArgs* p, void* stream) {
+    if (!p) return fail(MXK_ERR_BAD_ARG, "fp8_matmul: null arguments");
+    const int64_t rows = p->rows, cols = p->cols, depth = p->depth, experts = p->offsets ? p->experts : 1;
+    if (rows < 0 || cols < 1 || depth < 16 || depth % 16 || rows > (1 << 30) || depth > (1 << 30) || experts < 1 || experts > kMmMaxExperts || experts * cols > (1 << 30))
+        return fail(MXK_ERR_BAD_ARG, "fp8_matmul: need depth a multiple of 16, 1 <= experts <= 1024, rows and experts * cols <= 2^30");
+    if (p->x_format < MXK_FP8_E4M3 || p->x_format > MXK_FP8_E5M2 || p->w_format < MXK_FP8_E4M3 || p->w_format > MXK_FP8_E5M2)
+        return fail(MXK_ERR_BAD_ARG, "fp8_matmul: operand formats are MXK_FP8_E4M3 and MXK_FP8_E5M2");
+    if (rows == 0) return 0;
+    if (!p->x || !p->w || !p->out) return fail(MXK_ERR_BAD_ARG, "fp8_matmul: pointers must be non-null");
+    if ((addr(p->x) | addr(p->w) | (uint64_t)p->x_stride | (uint64_t)p->w_stride) & 15 || p->x_stride < depth || p->w_stride < depth)
+        return fail(MXK_ERR_BAD_ARG, "fp8_matmul: x and w need 16-byte aligned rows");
+    if ((addr(p->out) & 1) || (rows > 1 && p->out_stride < cols)) return fail(MXK_ERR_BAD_ARG, "fp8_matmul: out must be bf16 rows that do not overlap");
+    MmArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.x_sf = p->x_sf; a.w_sf = p->w_sf; a.out = p->out; a.offsets = p->offsets;
+    a.x_sf_stride = p->x_sf_stride; a.out_stride = p->out_stride;
+    a.rows = (int)rows; a.cols = (int)cols; a.nkb = (int)((depth + 127) / 128); a.experts = (int)experts;
+    a.w_per_row = p->w_sf_per_row ? 1 : 0;
+    a.w_sf_rows = a.w_per_row ? a.cols : (a.cols + 127) / 128;
+    a.zero_tail = p->offsets && p->zero_tail;
+    a.formats = ((uint32_t)p->w_format << 7) | ((uint32_t)p->x_format << 10);   // w is the MMA's A operand, x its B
+    a.wait_ns = p->max_spins > 0 ? (unsigned long long)p->max_spins * 250ull : 2000000000ull;
+
+    const int64_t mean = (rows + experts - 1) / experts;   // rows of a group, on average
+    const bool pair = mean > 128 && cols > 128;
+    const int groups = (a.nkb + 3) / 4;
+    a.splits = 1;
+    if (pair) {
+        a.n_tiles = (a.cols + 255) / 256;
+        a.bt_max = 240;
+        if (!p->offsets) {
+            // extent of a tile along x: the one whose last wave wastes least
+            double best = 1e30;
+            for (int bt = 240; bt >= 64; bt -= 16) {
+                const int64_t tt = (rows + bt - 1) / bt;
+                const int64_t real = ((rows + tt - 1) / tt + 15) / 16 * 16;
+                const int64_t waves = (tt * a.n_tiles + kSms / 2 - 1) / (kSms / 2);
+                const double cost = (double)waves * ((double)std::max<int64_t>(real, 96) + 8.0);
+                if (cost < best) { best = cost; a.bt_max = bt; }
+            }
+        }
+        a.box = a.bt_max / 2;
+    } else {
+        a.n_tiles = (a.cols + 127) / 128;
+        a.bt_max = mean <= 32 ? (int)std::min<int64_t>(32, (mean + 15) / 16 * 16) : 128;
+        if (p->offsets) a.bt_max = mean <= 16 ? 32 : 128;
+        a.box = a.bt_max;
+        const int64_t tiles = (p->offsets ? std::min<int64_t>(experts, rows) : (rows + a.bt_max - 1) / a.bt_max) * a.n_tiles;
+        while (a.splits < 8 && tiles * a.splits * 2 <= kSms && a.splits * 2 <= groups) a.splits *= 2;
+    }
+    a.acc_stride = a.bt_max;
+    a.sf_slot_cols = pair ? 12 : 8;
+    a.sf_col = 2 * a.acc_stride;
+    a.sf_slots = std::min(kMmMaxSfSlots, (kMmTmemCols - a.sf_col) / a.sf_slot_cols);
+    const int stage = kMmWBytes + a.box * 128;
+    const int fixed = 1024 + a.sf_slots * kMmSfSlotBytes + (a.splits > 1 ? a.bt_max * 512 : 0) + (int)sizeof(MmSmem) + 2 * (a.experts + 1) * 4;
+    a.n_stages = std::min(kMmMaxStages, (kMmSmemLimit - fixed) / stage);
+    const int smem = fixed + a.n_stages * stage;
+    CUtensorMap tm_x, tm_w;
+    if (int rc = byte_map(&tm_x, p->x, rows, depth, p->x_stride, a.box)) return rc;
+    if (int rc = byte_map(&tm_w, p->w, experts * cols, depth, p->w_stride, 128)) return rc;
+    const void* fn = pair ? (const void*)k_matmul_pair : (const void*)k_matmul;
+    if (int rc = allow_smem(fn, pair ? 1 : 2, kMmSmemLimit)) return rc;
+    const int cluster = (pair ? 2 : 1) * a.splits;
+    const int64_t tiles_most = ((p->offsets ? std::min<int64_t>(experts, rows) : 0) + (rows + a.bt_max - 1) / a.bt_max) * a.n_tiles;
+    if (tiles_most > (1 << 30)) return fail(MXK_ERR_BAD_ARG, "fp8_matmul: more than 2^30 tiles");
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(tiles_most, kSms / cluster) * cluster), 1, 1);
+    cfg.blockDim = dim3(kMmThreads, 1, 1);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = cluster; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+    cfg.attrs = &at; cfg.numAttrs = cluster > 1 ? 1 : 0;
+    const cudaError_t e = pair ? cudaLaunchKernelEx(&cfg, k_matmul_pair, a, tm_x, tm_w) : cudaLaunchKernelEx(&cfg, k_matmul, a, tm_x, tm_w);
+    return e == cudaSuccess ? 0 : cuda_fail(e, "launch k_matmul");
+}
+
+int mxk_matmul_status(int32_t* out) {
+    if (!out) return fail(MXK_ERR_BAD_ARG, "matmul_status: null argument");
+    int v = 0;
+    const cudaError_t e = cudaMemcpyFromSymbol(&v, g_mm_status, sizeof(v));
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMemcpyFromSymbol(matmul status)");
+    *out = v;
+    return 0;
+}
+
+}  // extern "C"

@@ -1,0 +1,280 @@
+"""8-bit products with block scales, dense and grouped, against 64-bit arithmetic on the dequantised operands.
+
+Tolerances.  `exact` cases use small integers and scales of 2^-2 .. 2^2: every product and partial sum is a multiple of
+2^-4 below 2^20, so FP32 holds all of them and only the rounding to bf16 is left: equal bits.
+Other cases: the tensor core adds the 32 products of one instruction and the accumulator after aligning them to
+the largest; each of the at most 33 terms loses less than 2^-23 of a value that is at most A = sum |x w|.  Over K / 32
+instructions that is at most 33 K / 32 * 2^-23 A, then one rounding of 2^-8: |d| <= 2^-8 |want| + 33 K / 32 * 2^-23 A (1 + 2^-8).
+"""
+import ctypes
+
+import pytest
+import torch
+
+import mini_mega_b200 as mm
+from mini_mega_b200 import _lib, matmul
+
+E4, E5 = torch.float8_e4m3fn, torch.float8_e5m2
+
+
+# ------------------------------------------------------------------------------ refusals
+def _x(rows=4, depth=256, dtype=E4):
+    return torch.zeros((rows, depth), dtype=dtype)
+
+
+def _sf(*shape):
+    return torch.full(shape, 127, dtype=torch.uint8)
+
+
+_OFF = torch.zeros(4, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("make, err", [
+    (lambda: mm.fp8_matmul(torch.zeros(4, 256), _x()), TypeError),
+    (lambda: mm.fp8_matmul(_x(), torch.zeros(4, 256, dtype=torch.bfloat16)), TypeError),
+    (lambda: mm.fp8_matmul((_x(), torch.ones(4, 2)), _x()), TypeError),
+    (lambda: mm.fp8_matmul(_x(depth=128), _x()), ValueError),
+    (lambda: mm.fp8_matmul(_x(depth=120), _x(depth=120)), ValueError),
+    (lambda: mm.fp8_matmul(_x(depth=0), _x(depth=0)), ValueError),
+    (lambda: mm.fp8_matmul(_x(), _x(rows=0)), ValueError),
+    (lambda: mm.fp8_matmul(_x()[0], _x()), ValueError),
+    (lambda: mm.fp8_matmul((_x(), _sf(4, 3)), _x()), ValueError),
+    (lambda: mm.fp8_matmul((_x(), _sf(2, 4).t()), _x()), ValueError),
+    (lambda: mm.fp8_matmul(_x(), (_x(rows=300), _sf(2, 2))), ValueError),
+    (lambda: mm.fp8_matmul(_x(), (_x(rows=300), _sf(2, 3).t())), ValueError),
+    (lambda: mm.fp8_matmul(_x(depth=512)[:, ::2], _x()), ValueError),
+    (lambda: mm.fp8_matmul(_x(depth=264)[:, :256], _x()), ValueError),
+    (lambda: mm.fp8_matmul(_x(depth=272)[:, 8:264], _x()), ValueError),
+    (lambda: mm.fp8_matmul(_x(rows=1).expand(4, 256), _x()), ValueError),
+    (lambda: mm.fp8_matmul(_x(), _x(), out=torch.zeros(4, 4)), ValueError),
+    (lambda: mm.fp8_matmul(_x(), _x(), out=torch.zeros((4, 5), dtype=torch.bfloat16)), ValueError),
+    (lambda: mm.fp8_matmul(_x(), _x(), out=torch.zeros((4, 8), dtype=torch.bfloat16)[:, ::2]), ValueError),
+    (lambda: mm.fp8_matmul(_x(), _x()), ValueError),                       # CPU tensors
+    (lambda: mm.fp8_grouped_matmul(_x(), _x(), _OFF), ValueError),         # w without an expert dimension
+    (lambda: mm.fp8_grouped_matmul(_x(), torch.zeros((3, 8, 256), dtype=E4), None), TypeError),
+    (lambda: mm.fp8_grouped_matmul(_x(), torch.zeros((4, 8, 256), dtype=E4), _OFF), ValueError),
+    (lambda: mm.fp8_grouped_matmul(_x(), torch.zeros((3, 8, 256), dtype=E4), _OFF.long()), ValueError),
+    (lambda: mm.fp8_grouped_matmul(_x(), torch.zeros((6, 8, 256), dtype=E4)[::2], _OFF), ValueError),
+    (lambda: mm.fp8_grouped_matmul(_x(), (torch.zeros((3, 8, 256), dtype=E4), _sf(1, 2)), _OFF), ValueError),
+    (lambda: mm.fp8_grouped_matmul(_x(), torch.zeros((3, 8, 256), dtype=E4), _OFF), ValueError),
+])
+def test_refusals(make, err):
+    with pytest.raises(err):
+        make()
+
+
+def test_packed_arguments_match_the_header(tmp_path):
+    """The struct format of matmul.py against MxkMatmulArgs as gcc lays it out."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = tmp_path / "s.c"
+    names = ["x", "x_sf", "w", "w_sf", "out", "offsets", "x_stride", "x_sf_stride", "w_stride", "out_stride", "rows", "cols",
+             "depth", "experts", "x_format", "w_format", "w_sf_per_row", "zero_tail", "max_spins"]
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "mxk_b200.h"\nint main(void) {\n  printf("%zu", sizeof(MxkMatmulArgs));\n'
+                   + "".join(f'  printf(" %zu", offsetof(MxkMatmulArgs, {n}));\n' for n in names) + "  return 0;\n}\n")
+    subprocess.run(["gcc", "-I", os.path.join(root, "include"), "-o", str(tmp_path / "s"), str(src)], check=True)
+    got = [int(v) for v in subprocess.run([str(tmp_path / "s")], check=True, capture_output=True, text=True).stdout.split()]
+    assert got == [matmul._ARGS.size] + [8 * i for i in range(10)] + [80 + 4 * i for i in range(9)]
+
+
+def test_c_abi_refuses_before_it_launches():
+    _lib.build()
+    L = _lib.lib()
+    good = dict(x=16, x_sf=0, w=16, w_sf=0, out=16, offsets=0, xs=128, xss=0, ws=128, os=8, rows=4, cols=8, depth=128, experts=1,
+                xf=0, wf=0, per_row=0, tail=0, spins=0)
+    for change in (dict(x=0), dict(w=0), dict(out=0), dict(rows=-1), dict(cols=0), dict(depth=120), dict(depth=8), dict(xs=112),
+                   dict(ws=136), dict(x=24), dict(out=17), dict(os=7), dict(xf=2), dict(wf=5), dict(offsets=16, experts=1025)):
+        assert L.mxk_fp8_matmul(matmul._ARGS.pack(*{**good, **change}.values()), None) == -1, change
+        assert b"fp8_matmul" in L.mxk_last_error()
+    assert L.mxk_fp8_matmul(None, None) == -1
+    assert L.mxk_matmul_status(ctypes.POINTER(ctypes.c_int32)()) == -1
+
+
+# ------------------------------------------------------------------------------- products
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _data(g, shape, dtype, exact):
+    if exact:
+        return torch.randint(-3, 4, shape, generator=g, device="cuda").float().to(dtype)
+    return (torch.randn(shape, generator=g, device="cuda") * 60).clamp(-440, 440).to(dtype)
+
+
+def _scales(g, shape, exact):
+    return torch.randint(126 if exact else 110, 129 if exact else 140, shape, generator=g, device="cuda", dtype=torch.uint8)
+
+
+def _dequant(q, sf, block_rows):
+    v = q.double()
+    if sf is None:
+        return v
+    f = torch.exp2(sf.double() - 127).repeat_interleave(128, -1)[..., :q.shape[-1]]
+    return v * (f.repeat_interleave(128, -2)[..., :q.shape[-2], :] if block_rows else f)
+
+
+def _check(out, a, b, exact):
+    want = a @ b.t()
+    if exact:
+        assert torch.equal(out, want.to(torch.bfloat16))
+        return
+    mass = a.abs() @ b.abs().t()
+    tol = 2.0 ** -8 * want.abs() + 33 * a.shape[1] / 32 * 2.0 ** -23 * mass * (1 + 2.0 ** -8)
+    d = (out.double() - want).abs()
+    assert bool((d <= tol).all()), f"{int((d > tol).sum())} of {d.numel()} off, worst by {float((d / tol).max()):.3g}"
+
+
+DENSE = [(1, 128, 128), (1, 4096, 2048), (1, 1, 16), (3, 130, 144), (16, 512, 6144), (17, 384, 640), (32, 100, 1040), (33, 256, 512),
+         (64, 640, 4096), (100, 1000, 272), (128, 2048, 384), (129, 257, 128), (200, 128, 1024), (240, 512, 512), (241, 300, 656),
+         (500, 777, 2064), (1000, 1536, 768), (2500, 512, 144)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("exact", [True, False])
+@pytest.mark.parametrize("form", ["block", "row", "raw"])
+@pytest.mark.parametrize("rows, cols, depth", DENSE)
+def test_dense(rows, cols, depth, form, exact):
+    g = _gen(rows * 7 + cols + depth)
+    blocks = (depth + 127) // 128
+    x, w = _data(g, (rows, depth), E4, exact), _data(g, (cols, depth), E4, exact)
+    xs, ws = (None, None) if form == "raw" else (_scales(g, (rows, blocks), exact),
+                                                 _scales(g, (cols if form == "row" else (cols + 127) // 128, blocks), exact))
+    out = mm.fp8_matmul(x if xs is None else (x, xs), w if ws is None else (w, ws))
+    _check(out, _dequant(x, xs, False), _dequant(w, ws, form == "block"), exact)
+    assert mm.matmul_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("xt", [E4, E5])
+@pytest.mark.parametrize("wt", [E4, E5])
+@pytest.mark.parametrize("rows", [5, 300])
+def test_formats(xt, wt, rows):
+    g = _gen(rows)
+    x, w = _data(g, (rows, 400), xt, False), _data(g, (210, 400), wt, False)
+    xs, ws = _scales(g, (rows, 4), False), _scales(g, (210, 4), False)
+    _check(mm.fp8_matmul((x, xs), (w, ws)), _dequant(x, xs, False), _dequant(w, ws, False), False)
+    if wt == E4 and xt == E4:
+        assert torch.equal(mm.fp8_matmul((x.view(torch.uint8), xs), (w.view(torch.uint8), ws)), mm.fp8_matmul((x, xs), (w, ws)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [7, 200])
+def test_views_and_rows_that_must_not_change(rows):
+    g = _gen(rows + 1)
+    x, w = _data(g, (rows, 512 + 32), E4, True), _data(g, (300, 512 + 64), E4, True)
+    xs = _scales(g, (rows, 9), True)
+    ws = _scales(g, (3, 4), True)
+    out = torch.full((rows + 2, 300 + 3), 7.0, dtype=torch.bfloat16, device="cuda")
+    got = mm.fp8_matmul((x[:, 16:528], xs[:, 3:7]), (w[:, 48:560], ws), out=out[1:-1, 1:301])
+    assert got.data_ptr() == out[1:-1, 1:301].data_ptr()
+    _check(got, _dequant(x[:, 16:528], xs[:, 3:7], False), _dequant(w[:, 48:560], ws, True), True)
+    rest = out.clone()
+    rest[1:-1, 1:301] = 7.0
+    assert bool((rest == 7.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 150])
+def test_special_values(rows):
+    """NaN bytes reach exactly their row and column; the scale byte 255 is NaN; extreme scales multiply out."""
+    x, w = torch.ones((rows, 256), device="cuda").to(E4), torch.ones((140, 256), device="cuda").to(E4)
+    x.view(torch.uint8)[1, 200], w.view(torch.uint8)[130, 3] = 0x7F, 0x7F
+    out = mm.fp8_matmul(x, w)
+    nan = torch.zeros((rows, 140), dtype=torch.bool, device="cuda")
+    nan[1], nan[:, 130] = True, True
+    assert torch.equal(torch.isnan(out), nan) and bool((out[~nan] == 256).all())
+    x, w = torch.ones((rows, 256), device="cuda").to(E4), torch.ones((140, 256), device="cuda").to(E4)
+    xs, ws = torch.full((rows, 2), 127, dtype=torch.uint8, device="cuda"), torch.full((140, 2), 127, dtype=torch.uint8, device="cuda")
+    xs[2, 1] = 255
+    xs[0], ws[5] = 127 + 60, 127 - 100
+    out = mm.fp8_matmul((x, xs), (w, ws)).float()
+    assert bool(torch.isnan(out[2]).all()) and not bool(torch.isnan(out[:2]).any())
+    assert float(out[0, 0]) == 2.0 ** 68 and float(out[0, 5]) == 2.0 ** -32 and float(out[1, 5]) == 2.0 ** -92
+
+
+# -------------------------------------------------------------------------------- grouped
+GROUPED = [  # rows of every expert, behind: rows of nobody; cols, depth
+    ([5], 0, 128, 128), ([0, 0, 3], 0, 256, 256), ([1] * 32, 0, 384, 512), ([4, 0, 1, 30, 2, 0], 5, 200, 1040),
+    ([16, 17, 15, 33, 0, 47], 0, 512, 656), ([100, 3, 0, 260], 9, 300, 384), ([300, 241, 0, 17, 480, 1000], 3, 640, 272),
+    ([0, 0, 0], 7, 130, 128), ([2000, 1, 1], 0, 257, 144), ([50] * 70, 11, 128, 128), ([9, 700], 2, 130, 2064)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("exact", [True, False])
+@pytest.mark.parametrize("form", ["block", "row", "raw"])
+@pytest.mark.parametrize("counts, behind, cols, depth", GROUPED)
+def test_grouped(counts, behind, cols, depth, form, exact):
+    g = _gen(sum(counts) + cols)
+    rows, experts, blocks = sum(counts) + behind, len(counts), (depth + 127) // 128
+    x, w = _data(g, (rows, depth), E4, exact), _data(g, (experts, cols, depth), E4, exact)
+    xs = ws = None
+    if form != "raw":
+        xs = _scales(g, (rows, blocks), exact)
+        ws = _scales(g, (experts, cols if form == "row" else (cols + 127) // 128, blocks), exact)
+    offsets = torch.tensor([0] + counts, device="cuda").cumsum(0).int()
+    arg_x, arg_w = (x, w) if xs is None else ((x, xs), (w, ws))
+    out = mm.fp8_grouped_matmul(arg_x, arg_w, offsets)
+    given = torch.full((rows, cols), 7.0, dtype=torch.bfloat16, device="cuda")
+    mm.fp8_grouped_matmul(arg_x, arg_w, offsets, out=given)
+    a, r = _dequant(x, xs, False), 0
+    for e, n in enumerate(counts):
+        _check(out[r:r + n], a[r:r + n], _dequant(w[e], None if ws is None else ws[e], form == "block"), exact)
+        r += n
+    assert bool((out[r:] == 0).all()) and bool((given[r:] == 7.0).all()) and torch.equal(given[:r], out[:r])
+    assert mm.matmul_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("per_expert", [8, 60, 400])
+def test_wild_offsets_stay_inside(per_expert):
+    """Offsets out of range or out of order: clamped and made ascending, rows outside every group zero."""
+    g = _gen(per_expert)
+    rows, experts, cols, depth = per_expert * 5, 5, 192, 256
+    x, w = _data(g, (rows, depth), E4, True), _data(g, (experts, cols, depth), E4, True)
+    for raw in ([-9, rows // 3, rows // 4, rows // 2, rows + 50, 2 ** 31 - 1], [rows // 5, 7, -2 ** 31, rows // 2, rows // 2, rows - 1]):
+        off, top = [], 0
+        for v in raw:
+            top = max(top, min(max(v, 0), rows))
+            off.append(top)
+        out = mm.fp8_grouped_matmul(x, w, torch.tensor(raw, dtype=torch.int32, device="cuda"))
+        want = torch.zeros((rows, cols), dtype=torch.bfloat16, device="cuda")
+        for e in range(experts):
+            want[off[e]:off[e + 1]] = (x[off[e]:off[e + 1]].double() @ w[e].double().t()).to(torch.bfloat16)
+        assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+def test_captured_replayed_on_two_streams_and_without_rows():
+    g = _gen(2)
+    w = _data(g, (6, 640, 512), E4, False)
+    cases = [(_data(g, (40, 512), E4, False), torch.tensor([0, 9, 9, 20, 31, 31, 40], dtype=torch.int32, device="cuda")),
+             (_data(g, (1500, 512), E4, False), torch.tensor([0, 300, 301, 301, 900, 1200, 1480], dtype=torch.int32, device="cuda"))]
+    calls = [lambda x=x, o=o: mm.fp8_grouped_matmul(x, w, o) for x, o in cases] + [lambda x=x: mm.fp8_matmul(x, w[2]) for x, _ in cases]
+    want = [c() for c in calls]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    for c in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = c()
+        graphs.append((graph, held))
+    for _ in range(3):
+        for graph, _ in graphs:
+            graph.replay()
+        with torch.cuda.stream(side):
+            beside = [c() for c in calls]
+        here = [c() for c in calls]
+        torch.cuda.synchronize()
+        for i, (_, held) in enumerate(graphs):
+            assert torch.equal(held, want[i]) and torch.equal(beside[i], want[i]) and torch.equal(here[i], want[i])
+    # the offsets are read when the graph runs
+    offsets = cases[0][1]
+    offsets.copy_(torch.tensor([0, 0, 25, 25, 26, 40, 40], dtype=torch.int32))
+    graphs[0][0].replay()
+    assert torch.equal(graphs[0][1], mm.fp8_grouped_matmul(cases[0][0], w, offsets))
+    empty = torch.empty((0, 512), dtype=E4, device="cuda")
+    assert mm.fp8_matmul(empty, w[0]).shape == (0, 640)
+    assert mm.fp8_grouped_matmul(empty, w, torch.zeros(7, dtype=torch.int32, device="cuda")).shape == (0, 640)
+    assert mm.matmul_status() == 0
