@@ -1,4 +1,5 @@
-"""ctypes binding of libmxk_b200.so (the C ABI of include/mxk_b200.h).
+"""ctypes binding of libmxk_b200.so (the C ABI of include/mxk_b200.h), and the loader of _ops.so, the torch
+binding of the operators beside the layer.
 
 The CUDA library is the product path: if it is missing this module raises, it
 never falls back to a CPU implementation.
@@ -11,6 +12,7 @@ import subprocess
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmxk_b200.so")
+OPS_PATH = os.path.join(_HERE, "_ops.so")
 SRC_DIR = os.path.join(_HERE, "csrc")
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
@@ -24,12 +26,37 @@ def build(force: bool = False, verbose: bool = False) -> str:
     srcs = units + [os.path.join(SRC_DIR, f) for f in ("mxk_device.cuh", "mxk_phases.cuh", "mxk_gemm.cuh", "mxk_sched.cuh",
                                                        "mxk_rows.cuh", "mxk_matmul.cuh")]
     hdr = os.path.join(os.path.dirname(_HERE), "include", "mxk_b200.h")
-    newest = max(os.path.getmtime(p) for p in srcs + [hdr])
-    if not force and os.path.exists(LIB_PATH) and os.path.getmtime(LIB_PATH) >= newest:
+    if not force and _current(LIB_PATH, srcs + [hdr]):
+        build_ops(False)
         return LIB_PATH
     cmd = ["nvcc"] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["--threads", "2", "-o", LIB_PATH] + units
     subprocess.run(cmd, check=True)
+    build_ops(force)
     return LIB_PATH
+
+
+def _current(target: str, sources) -> bool:
+    return os.path.exists(target) and os.path.getmtime(target) >= max(os.path.getmtime(p) for p in sources)
+
+
+def build_ops(force: bool = False) -> str:
+    """Compile csrc/mxk_torch.cpp into _ops.so next to the library, which it links."""
+    import sysconfig
+
+    import torch
+    src = os.path.join(SRC_DIR, "mxk_torch.cpp")
+    hdr = os.path.join(os.path.dirname(_HERE), "include", "mxk_b200.h")
+    if not force and _current(OPS_PATH, [src, hdr]):
+        return OPS_PATH
+    at = os.path.dirname(torch.__file__)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    include = [os.path.join(at, "include"), os.path.join(at, "include", "torch", "csrc", "api", "include"),
+               os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared"] + [f for d in include for f in ("-isystem", d)]
+    cmd += ["-o", OPS_PATH, src, "-L" + os.path.join(at, "lib"), "-L" + _HERE, "-l:libmxk_b200.so", "-ltorch", "-ltorch_cpu",
+            "-ltorch_cuda", "-ltorch_python", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    subprocess.run(cmd, check=True)
+    return OPS_PATH
 
 
 class MxkGeom(C.Structure):
@@ -77,6 +104,13 @@ class MxkLaunchArgs(C.Structure):
     ]
 
 
+class MxkMatmulArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "x_sf", "w", "w_sf", "out", "offsets")] + \
+               [(n, C.c_int64) for n in ("x_stride", "x_sf_stride", "w_stride", "out_stride")] + \
+               [(n, C.c_int32) for n in ("rows", "cols", "depth", "experts", "x_format", "w_format", "w_sf_per_row", "zero_tail",
+                                         "max_spins")]
+
+
 class MxkStatus(C.Structure):
     _fields_ = [("launches", C.c_int64), ("status", C.c_int32), ("n_tasks", C.c_int32), ("n_l1_tasks", C.c_int32),
                 ("n_windows", C.c_int32), ("total_rows", C.c_int32), ("helper_on", C.c_int32), ("dbg", C.c_int32 * 8),
@@ -96,6 +130,7 @@ EXPORTS = [
 ]
 
 _LIB = None
+_OPS = None
 
 
 class MxkError(RuntimeError):
@@ -144,7 +179,7 @@ def lib():
     L.mxk_sort_tokens.argtypes = [vp, i64, i64, vp, i64, i64, i32, i32, i32, vp, vp, vp, vp, vp]
     L.mxk_unsort_tokens.argtypes = [vp, i32, i64, vp, i64, i32, i32, i32, vp, vp, vp]
     L.mxk_unsort_tokens_grad.argtypes = [vp, i64, vp, i64, i32, vp, i64, i32, i32, i32, i32, vp, vp, vp, vp, vp]
-    L.mxk_fp8_matmul.argtypes = [C.c_char_p, vp]     # a packed MxkMatmulArgs
+    L.mxk_fp8_matmul.argtypes = [C.POINTER(MxkMatmulArgs), vp]
     L.mxk_matmul_status.argtypes = [C.POINTER(C.c_int32)]
     L.mxk_symm_alloc.argtypes = [C.POINTER(C.c_void_p), C.c_int64]
     L.mxk_symm_free.argtypes = [C.c_void_p]
@@ -153,6 +188,17 @@ def lib():
     L.mxk_ipc_close.argtypes = [C.c_void_p]
     _LIB = L
     return L
+
+
+def ops():
+    """The torch binding of the operators; raises if it has not been built."""
+    global _OPS
+    if _OPS is None:
+        if not os.path.exists(OPS_PATH) or not os.path.exists(LIB_PATH):
+            raise MxkError(f"{OPS_PATH} is missing: run mini_mega_b200._lib.build() (needs nvcc); there is no CPU fallback")
+        import importlib
+        _OPS = importlib.import_module("mini_mega_b200._ops")
+    return _OPS
 
 
 def check(rc: int, what: str = "") -> None:

@@ -85,13 +85,13 @@ int byte_map(CUtensorMap* m, const void* base, int64_t rows, int64_t k, int64_t 
 // Work split of the row kernels: `span` whole rows per CTA of narrow rows, column parts of one row
 // when rows are wide or few.
 struct RowGrid { int span, vecs, part_vecs, threads; dim3 grid; };
-RowGrid row_grid(int tokens, int row_bytes, int vec) {
+RowGrid row_grid(int tokens, int row_bytes, int vec, int per_cta) {
     RowGrid g;
     g.vecs = row_bytes / vec;
-    g.span = std::max(1, 512 / g.vecs);
+    g.span = std::max(1, per_cta / g.vecs);
     g.part_vecs = g.vecs;
     if (g.span == 1) {
-        const int parts_min = (g.vecs + 1023) / 1024;
+        const int parts_min = (g.vecs + per_cta - 1) / per_cta;
         const int parts_fill = std::min((g.vecs + 63) / 64, (2 * kSms + tokens - 1) / tokens);   // few tokens: more CTAs per row
         const int parts = std::min(65535, std::max(parts_min, parts_fill));
         g.part_vecs = (g.vecs + parts - 1) / parts;
@@ -184,7 +184,7 @@ int mxk_sort_tokens(const void* x, int64_t x_stride, int64_t row_bytes, const vo
         const int v = common_vec(addr(x_sf) | addr(rows_sf) | (uint64_t)sf_stride | (uint64_t)sf_bytes);
         a.sf_vec = v == 2 ? 1 : v;
     }
-    const RowGrid g = row_grid(tokens, a.row_bytes, vec);
+    const RowGrid g = row_grid(tokens, a.row_bytes, vec, 1024);
     a.tokens = tokens; a.topk = topk; a.pairs = tokens * topk; a.span = g.span; a.vecs = g.vecs; a.part_vecs = g.part_vecs;
     a.fvecs = FastDiv::make((uint32_t)g.vecs);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -210,7 +210,7 @@ int mxk_unsort_tokens(const void* rows, int32_t dtype, int64_t rows_stride, cons
     a.rows_stride = rows_stride; a.w_stride = weights_stride; a.row_bytes = hidden * dtype_bytes(dtype);
     const int vec = common_vec(addr(rows) | addr(y) | (uint64_t)rows_stride | (uint64_t)a.row_bytes);
     if (vec < dtype_bytes(dtype)) return fail(MXK_ERR_BAD_ARG, "unsort_tokens: rows and y must be aligned to their element type");
-    const RowGrid g = row_grid(tokens, a.row_bytes, vec);
+    const RowGrid g = row_grid(tokens, a.row_bytes, vec, 256);
     a.tokens = tokens; a.topk = topk; a.pairs = tokens * topk; a.span = g.span; a.vecs = g.vecs; a.part_vecs = g.part_vecs;
     a.fvecs = FastDiv::make((uint32_t)g.vecs);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -248,7 +248,7 @@ struct UnsortArgs {
 };
 
 template <int kType, int V>
-__global__ void __launch_bounds__(256) k_unsort_rows(const UnsortArgs a) {
+__global__ void __launch_bounds__(256, 4) k_unsort_rows(const UnsortArgs a) {
     constexpr int kEl = elem_bytes<kType>(), kN = V / kEl;
     typedef typename VecOf<V>::T T;
     const int t0 = (int)blockIdx.x * a.span;
@@ -267,11 +267,11 @@ __global__ void __launch_bounds__(256) k_unsort_rows(const UnsortArgs a) {
             float w[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int r = j0 + j < a.topk ? rp[j0 + j] : -1;
+                const int r = j0 + j < a.topk ? __ldg(rp + j0 + j) : -1;
                 const bool ok = r >= 0 && r < a.pairs;
-                w[j] = ok ? (a.w ? a.w[t * a.w_stride + j0 + j] : 1.0f) : 0.0f;
+                w[j] = ok ? (a.w ? __ldg(a.w + t * a.w_stride + j0 + j) : 1.0f) : 0.0f;
                 memset(&v[j], 0, sizeof(T));     // a dropped pair adds nothing, whatever its row holds
-                if (ok) v[j] = *reinterpret_cast<const T*>(a.rows + (long long)r * a.rows_stride + at);
+                if (ok) v[j] = __ldg(reinterpret_cast<const T*>(a.rows + (long long)r * a.rows_stride + at));
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j)

@@ -274,6 +274,23 @@ def test_gradients_against_differences():
 
 
 @pytest.mark.gpu
+def test_second_derivatives():
+    """Sort and plain unsort are linear: differentiating their gradients again works; the weighted sum refuses."""
+    plan = table_device(routing(4, 6, 3, 4, 0.2), 4)
+    x = torch.randn(6, 20, device="cuda", requires_grad=True)
+    c = torch.randn(6, 20, device="cuda", requires_grad=True)
+    y = mm.unsort_tokens_by_expert(mm.sort_tokens_by_expert(x, plan), plan)       # x times its number of kept pairs
+    gx, = torch.autograd.grad(y, x, c, create_graph=True)
+    kept = (plan.row_of_pair >= 0).sum(1, keepdim=True).float()
+    gc, = torch.autograd.grad(gx.sum(), c)
+    assert torch.equal(gc, kept.expand(6, 20))
+    rows = torch.randn(18, 20, device="cuda", requires_grad=True)
+    y = mm.unsort_tokens_by_expert(rows, plan, torch.rand(6, 3, device="cuda"))
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(y, rows, c, create_graph=True)
+
+
+@pytest.mark.gpu
 def test_masked_places_do_not_matter():
     """NaN and infinity behind the last row, and in rows and tokens whose pairs are dropped, reach no result."""
     idx = routing(12, 16, 4, 6, 0.3)

@@ -12,7 +12,7 @@ import pytest
 import torch
 
 import mini_mega_b200 as mm
-from mini_mega_b200 import _lib, matmul
+from mini_mega_b200 import _lib
 
 E4, E5 = torch.float8_e4m3fn, torch.float8_e5m2
 
@@ -63,32 +63,31 @@ def test_refusals(make, err):
         make()
 
 
-def test_packed_arguments_match_the_header(tmp_path):
-    """The struct format of matmul.py against MxkMatmulArgs as gcc lays it out."""
+def test_ctypes_mirror_matches_the_header(tmp_path):
+    """Size and field offsets of MxkMatmulArgs as gcc lays it out against the ctypes mirror."""
     import os
     import subprocess
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    src = tmp_path / "s.c"
-    names = ["x", "x_sf", "w", "w_sf", "out", "offsets", "x_stride", "x_sf_stride", "w_stride", "out_stride", "rows", "cols",
-             "depth", "experts", "x_format", "w_format", "w_sf_per_row", "zero_tail", "max_spins"]
+    src, args = tmp_path / "s.c", _lib.MxkMatmulArgs
+    names = [f[0] for f in args._fields_]
     src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "mxk_b200.h"\nint main(void) {\n  printf("%zu", sizeof(MxkMatmulArgs));\n'
                    + "".join(f'  printf(" %zu", offsetof(MxkMatmulArgs, {n}));\n' for n in names) + "  return 0;\n}\n")
     subprocess.run(["gcc", "-I", os.path.join(root, "include"), "-o", str(tmp_path / "s"), str(src)], check=True)
     got = [int(v) for v in subprocess.run([str(tmp_path / "s")], check=True, capture_output=True, text=True).stdout.split()]
-    assert got == [matmul._ARGS.size] + [8 * i for i in range(10)] + [80 + 4 * i for i in range(9)]
+    assert got == [ctypes.sizeof(args)] + [getattr(args, n).offset for n in names]
 
 
 def test_c_abi_refuses_before_it_launches():
     _lib.build()
     L = _lib.lib()
-    good = dict(x=16, x_sf=0, w=16, w_sf=0, out=16, offsets=0, xs=128, xss=0, ws=128, os=8, rows=4, cols=8, depth=128, experts=1,
-                xf=0, wf=0, per_row=0, tail=0, spins=0)
-    for change in (dict(x=0), dict(w=0), dict(out=0), dict(rows=-1), dict(cols=0), dict(depth=120), dict(depth=8), dict(xs=112),
-                   dict(ws=136), dict(x=24), dict(out=17), dict(os=7), dict(xf=2), dict(wf=5), dict(offsets=16, experts=1025)):
-        assert L.mxk_fp8_matmul(matmul._ARGS.pack(*{**good, **change}.values()), None) == -1, change
+    good = dict(x=16, w=16, out=16, x_stride=128, w_stride=128, out_stride=8, rows=4, cols=8, depth=128, experts=1)
+    for change in (dict(x=0), dict(w=0), dict(out=0), dict(rows=-1), dict(cols=0), dict(depth=120), dict(depth=8), dict(x_stride=112),
+                   dict(w_stride=136), dict(x=24), dict(out=17), dict(out_stride=7), dict(x_format=2), dict(w_format=5),
+                   dict(offsets=16, experts=1025)):
+        assert L.mxk_fp8_matmul(ctypes.byref(_lib.MxkMatmulArgs(**{**good, **change})), None) == -1, change
         assert b"fp8_matmul" in L.mxk_last_error()
     assert L.mxk_fp8_matmul(None, None) == -1
-    assert L.mxk_matmul_status(ctypes.POINTER(ctypes.c_int32)()) == -1
+    assert L.mxk_matmul_status(None) == -1
 
 
 # ------------------------------------------------------------------------------- products
