@@ -20,8 +20,10 @@
 // on several streams or in several graphs share nothing.
 //
 // Warp roles (384 threads) as in the layer's GEMM phase: warp 0 TMA producer, warp 1 MMA issuer,
-// warps 2-3 scale tiles (global bytes -> shared tile -> tensor memory), warps 4-11 epilogue.  Two
-// accumulators alternate, so the drain of one tile hides under the MMAs of the next.
+// warps 2-3 scale tiles (global bytes -> shared tile -> tensor memory), warps 4-11 epilogue.  Tensor
+// memory holds two accumulators of up to 224 columns that alternate between tiles, so that the drain
+// of one hides under the MMAs of the next.  (Both as the halves of one tile of 448 rows were slower, although a
+// quarter fewer bytes cross L2: MMAs that alternate between two accumulators ran at 75 % of the pipe.)
 //
 // Few tiles (small batches): the K extent is split over the CTAs of a cluster, the partial tiles
 // are exchanged through distributed shared memory and added in the order of the splits, so results
@@ -34,10 +36,12 @@
 constexpr int kMmThreads = 384;
 constexpr int kMmEpiWarps = 8;
 constexpr int kMmFirstEpi = 4;
-constexpr int kMmMaxStages = 12;
+constexpr int kMmMaxStages = 8;
 constexpr int kMmMaxSfSlots = 8;
 constexpr int kMmSfTile = 512;                 // 128 rows x 4 scale bytes
-constexpr int kMmSfSlotBytes = 3 * kMmSfTile;  // weight rows, x rows 0-127, x rows 128-255
+constexpr int kMmStageKb = 2, kMmPairStageKb = 2;   // K blocks of a ring stage
+constexpr int kMmRowsMax = 224;                // columns of an accumulator: 2 x 224 leave 64 TMEM columns to the scales
+constexpr int kMmChunks = kMmRowsMax / 16 / 2;  // 16-column chunks a warp drains of one accumulator
 constexpr int kMmWBytes = 128 * 128;           // weight tile of one K block
 constexpr int kMmMaxExperts = 1024;
 constexpr int kMmTmemCols = 512;
@@ -51,8 +55,8 @@ struct MmArgs {
     long long x_sf_stride, out_stride;
     int rows, cols, nkb, experts;
     int n_tiles;               // weight tiles of a group
-    int bt_max, box;           // rows of x per tile at most; rows per TMA box (pairs: half a tile)
-    int n_stages, sf_slots, acc_stride, sf_col, sf_slot_cols;
+    int bt_max, box;           // rows of x per tile at most; rows per TMA box (pairs: half of them)
+    int n_stages, sf_slots, sf_col;
     int splits;                // CTAs (pairs) of a cluster that share a tile's K extent
     int w_sf_rows, w_per_row;  // rows of a group's weight scale plane; 1: one scale row per weight row
     int zero_tail;             // clear out rows behind the last group
@@ -70,7 +74,7 @@ struct MmSmem {
 };
 
 struct MmTile {
-    int group, w_row, x_row, bt, valid;   // w_row: first weight row inside the group; x_row: first row of x
+    int group, w_row, x_row, bt, valid;    // w_row: first weight row inside the group; x_row, bt: rows of x
 };
 
 // status word of the products on this device: 0, or the first wait that expired
@@ -90,7 +94,7 @@ __device__ __forceinline__ bool mm_tile(const MmArgs& a, const int* start, const
     const bool rows_fast = n <= a.cols;
     const int xt = rows_fast ? i % tt : i / a.n_tiles, wt = rows_fast ? i / tt : i % a.n_tiles;
     o.group = lo;
-    o.bt = (((n + tt - 1) / tt) + 15) & ~15;
+    o.bt = ((n + tt - 1) / tt + 15) & ~15;   // the group's rows spread evenly over its tiles
     o.w_row = wt * (kPair ? 256 : 128);
     o.x_row = start[lo] + xt * o.bt;
     o.valid = min(o.bt, n - xt * o.bt);
@@ -116,6 +120,11 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+    return p != 0;
+}
 // commit of a pair's MMAs onto the barrier at this offset in both CTAs of the pair that starts at
 // cluster rank `first` (a signal inside one cluster; no load, no other GPU's memory)
 __device__ __forceinline__ void umma_commit_pair_at(uint32_t bar_smem_addr, uint32_t first) {
@@ -124,13 +133,16 @@ __device__ __forceinline__ void umma_commit_pair_at(uint32_t bar_smem_addr, uint
                  : "memory");
 }
 
-template <bool kPair>
+template <bool kPair, int kStageKb>   // kStageKb: K blocks of a ring stage
 __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x, const CUtensorMap* tm_w) {
     extern __shared__ uint8_t mm_smem_raw[];
     uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(mm_smem_raw) + 1023) & ~(uintptr_t)1023);
-    const uint32_t stage_bytes = (uint32_t)kMmWBytes + (uint32_t)a.box * 128u;
+    constexpr int kXTiles = kPair ? 2 : 1, kSfTiles = 1 + kXTiles;   // scale tiles: weight rows, then 128 rows of x each
+    constexpr uint32_t kSfSlotBytes = kSfTiles * kMmSfTile, kSfSlotCols = kSfTiles * 4;
+    const uint32_t x_bytes = (uint32_t)a.box * 128u;
+    const uint32_t stage_bytes = (uint32_t)kStageKb * ((uint32_t)kMmWBytes + x_bytes);   // [w]..[x].., tiles of 128-byte rows
     uint8_t* sf_tiles = tiles + (size_t)a.n_stages * stage_bytes;
-    float* red = reinterpret_cast<float*>(sf_tiles + a.sf_slots * kMmSfSlotBytes);   // [bt_max][128], splits > 1 only
+    float* red = reinterpret_cast<float*>(sf_tiles + a.sf_slots * kSfSlotBytes);   // [bt_max][128], splits > 1 only
     MmSmem* S = reinterpret_cast<MmSmem*>(reinterpret_cast<uint8_t*>(red) + (a.splits > 1 ? (size_t)a.bt_max * 512 : 0));
     int* start = reinterpret_cast<int*>(S + 1);
     int* before = start + a.experts + 1;  // both [experts + 1]
@@ -221,24 +233,33 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
             uint32_t stage = 0, phase = 0;
             unsigned long long issued = 0;
             bool dead = false;
-            const uint32_t tx = ctas * stage_bytes;
             for (int t = unit; !dead && mm_tile<kPair>(a, start, before, t, tl); t += n_units) {
                 // rows of all experts lie behind one another in the weight map; a tile that runs past its
                 // expert's last row reads the next expert's, and those output columns are not stored
                 const int w_row = (int)((long long)tl.group * a.cols) + tl.w_row + 128 * (int)half;
                 const int x_row = tl.x_row + (kPair ? (int)half * (tl.bt >> 1) : 0);
-                for (int kb = kb_first; kb < kb_last; ++kb) {
+                for (int kb = kb_first; kb < kb_last; kb += kStageKb) {
                     if (!mbar_wait(&S->empty[stage], phase ^ 1, wait_ns, abort_flag)) { dead = true; break; }
                     uint8_t* sw = tiles + (size_t)stage * stage_bytes;
+                    uint8_t* sx = sw + kStageKb * kMmWBytes;
+                    const bool two = kStageKb == 2 && kb + 1 < kb_last;
+                    const uint32_t tx = ctas * ((uint32_t)kMmWBytes + x_bytes) * (two ? 2u : 1u);
+                    uint32_t bar = 0;
                     if constexpr (kPair) {
                         if (leader) mbar_expect_tx(&S->full[stage], tx);
-                        const uint32_t bar = mapa_u32(smem_u32(&S->full[stage]), first);
-                        tma_load_2d_pair(sw, tm_w, kb * 128, w_row, bar);
-                        tma_load_2d_pair(sw + kMmWBytes, tm_x, kb * 128, x_row, bar);
+                        bar = mapa_u32(smem_u32(&S->full[stage]), first);
                     } else {
                         mbar_expect_tx(&S->full[stage], tx);
-                        tma_load_2d(sw, tm_w, kb * 128, w_row, &S->full[stage]);
-                        tma_load_2d(sw + kMmWBytes, tm_x, kb * 128, x_row, &S->full[stage]);
+                    }
+                    auto load = [&](uint8_t* dst, const CUtensorMap* map, int k, int row) {
+                        if constexpr (kPair) tma_load_2d_pair(dst, map, k * 128, row, bar);
+                        else tma_load_2d(dst, map, k * 128, row, &S->full[stage]);
+                    };
+                    load(sw, tm_w, kb, w_row);
+                    load(sx, tm_x, kb, x_row);
+                    if (two) {
+                        load(sw + kMmWBytes, tm_w, kb + 1, w_row);
+                        load(sx + x_bytes, tm_x, kb + 1, x_row);
                     }
                     ++issued;
                     if (++stage == (uint32_t)a.n_stages) { stage = 0; phase ^= 1; }
@@ -254,59 +275,73 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
         }
     } else if (warp == 1) {
         // ----------------------------------------------------------------- MMA issuer
-        if (lane == 0 && leader) {
-            uint32_t stage = 0, phase = 0, sfg = 0, it = 0;
-            bool stage_ready = false, dead = false;
+        // The whole warp walks the loop, one elected lane issues: descriptors and barrier addresses
+        // stay warp-uniform, which keeps the issue path short.  It has to be: a K block of a 256 x 208 tile is 416
+        // tensor-pipe cycles, the pipe queues only a few MMAs, and every wait and commit costs this warp on the
+        // order of 100 cycles.  Hence two K blocks per stage (one wait, one commit for eight MMAs) and waits at
+        // CTA scope wherever a commit is what arrives (one wait at cluster scope took 290 cycles).
+        if (leader) {
+            uint32_t stage = 0, phase = 0, slot = 0, slot_phase = 0, it = 0;
+            bool dead = false;
+            const bool elected = elect_one();
             const uint64_t desc0 = umma_smem_desc_sw128(smem_u32(tiles));
-            const uint32_t desc_step = stage_bytes >> 4;
+            const uint32_t w_step = (uint32_t)kMmWBytes >> 4, x_step = x_bytes >> 4, desc_step = stage_bytes >> 4;
+            const uint32_t n_stages = (uint32_t)a.n_stages, sf_slots = (uint32_t)a.sf_slots;
+            auto warp_wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+                if (__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity) ? 1 : 0)) return true;
+                return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, wait_ns, abort_flag) ? 1 : 0) != 0;
+            };
+            auto mma = [&](uint32_t d, uint64_t wdesc, uint64_t xdesc, uint32_t idesc, uint32_t tsf, uint32_t acc) {
+                if constexpr (kPair) umma_mxf8_pair(d, wdesc, xdesc, idesc, tsf, tsf + 4, acc);
+                else umma_mxf8(d, wdesc, xdesc, idesc, tsf, tsf + 4, acc);
+            };
+            auto commit = [&](uint64_t* bar) {
+                if constexpr (kPair) umma_commit_pair_at(smem_u32(bar), first);
+                else umma_commit(bar);
+            };
             for (int t = unit; !dead && mm_tile<kPair>(a, start, before, t, tl); t += n_units, ++it) {
-                const uint32_t buf = it & 1u, use = it >> 1;
-                if (!wait_bar(&S->acc_empty[buf], (use & 1u) ^ 1u)) { dead = true; break; }
                 const uint32_t idesc0 = umma_idesc_mx_e4m3(kPair ? 256 : 128, tl.bt, 0, 0) | a.formats;
-                const uint32_t tacc = tmem_base + buf * (uint32_t)a.acc_stride;
+                const uint32_t buf = it & 1u, use = it >> 1;
+                const uint32_t tacc = tmem_base + buf * (uint32_t)a.bt_max;
+                // the epilogue must have drained this accumulator's previous tile
+                if (!__all_sync(0xFFFFFFFFu, wait_bar(&S->acc_empty[buf], (use & 1u) ^ 1u) ? 1 : 0)) { dead = true; break; }
+                tc_fence_after();
                 uint32_t acc = 0;
-                for (int kb0 = kb_first; kb0 < kb_last && !dead; kb0 += 4) {
-                    const uint32_t slot = sfg % (uint32_t)a.sf_slots;
-                    if (!wait_bar(&S->sf_full[slot], (sfg / (uint32_t)a.sf_slots) & 1u)) { dead = true; break; }
-                    const uint32_t tsf = tmem_base + (uint32_t)a.sf_col + slot * (uint32_t)a.sf_slot_cols;
+                for (int kb0 = kb_first; kb0 < kb_last; kb0 += 4) {
+                    if (!warp_wait(&S->sf_full[slot], slot_phase)) { dead = true; break; }
+                    const uint32_t tsf = tmem_base + (uint32_t)a.sf_col + slot * kSfSlotCols;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < 4; i += kStageKb) {
                         if (kb0 + i >= kb_last) break;
-                        if (!stage_ready && !wait_bar(&S->full[stage], phase)) { dead = true; break; }
+                        if (!warp_wait(&S->full[stage], phase)) { dead = true; break; }
                         tc_fence_after();
                         const uint64_t wdesc = desc0 + (uint64_t)(stage * desc_step);
-                        const uint64_t xdesc = wdesc + (uint64_t)(kMmWBytes >> 4);
-                        const uint32_t idesc = idesc0 | ((uint32_t)i << 4) | ((uint32_t)i << 29);   // scale byte i of the group
-                        uint32_t nstage = stage + 1, nphase = phase;
-                        if (nstage == (uint32_t)a.n_stages) { nstage = 0; nphase ^= 1; }
-                        if constexpr (kPair) {
-                            umma_mxf8_pair(tacc, wdesc, xdesc, idesc, tsf, tsf + 4, acc);
-                            umma_mxf8_pair(tacc, wdesc + 2, xdesc + 2, idesc, tsf, tsf + 4, 1u);
-                            stage_ready = mbar_try_wait_cluster(&S->full[nstage], nphase);   // polled under the MMAs already queued
-                            umma_mxf8_pair(tacc, wdesc + 4, xdesc + 4, idesc, tsf, tsf + 4, 1u);
-                            umma_mxf8_pair(tacc, wdesc + 6, xdesc + 6, idesc, tsf, tsf + 4, 1u);
-                            umma_commit_pair_at(smem_u32(&S->empty[stage]), first);
-                        } else {
-                            umma_mxf8(tacc, wdesc, xdesc, idesc, tsf, tsf + 4, acc);
-                            umma_mxf8(tacc, wdesc + 2, xdesc + 2, idesc, tsf, tsf + 4, 1u);
-                            stage_ready = mbar_try_wait(&S->full[nstage], nphase);
-                            umma_mxf8(tacc, wdesc + 4, xdesc + 4, idesc, tsf, tsf + 4, 1u);
-                            umma_mxf8(tacc, wdesc + 6, xdesc + 6, idesc, tsf, tsf + 4, 1u);
-                            umma_commit(&S->empty[stage]);
+                        const uint64_t xdesc = wdesc + (uint64_t)((kStageKb * kMmWBytes) >> 4);
+                        const uint32_t id0 = idesc0 | ((uint32_t)i << 4) | ((uint32_t)i << 29);        // scale byte i of the group
+                        const uint32_t id1 = idesc0 | ((uint32_t)(i + 1) << 4) | ((uint32_t)(i + 1) << 29);
+                        if (elected) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) mma(tacc, wdesc + 2 * k, xdesc + 2 * k, id0, tsf, k ? 1u : acc);
+                            if (kStageKb == 2 && kb0 + i + 1 < kb_last) {
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) mma(tacc, wdesc + w_step + 2 * k, xdesc + x_step + 2 * k, id1, tsf, 1u);
+                            }
+                            commit(&S->empty[stage]);
                         }
+                        __syncwarp();
                         acc = 1u;
-                        stage = nstage; phase = nphase;
+                        if (++stage == n_stages) { stage = 0; phase ^= 1; }
                     }
                     if (dead) break;
-                    if constexpr (kPair) umma_commit_pair_at(smem_u32(&S->sf_empty[slot]), first);
-                    else umma_commit(&S->sf_empty[slot]);
-                    ++sfg;
+                    if (elected) commit(&S->sf_empty[slot]);
+                    __syncwarp();
+                    if (++slot == sf_slots) { slot = 0; slot_phase ^= 1; }
                 }
                 if (dead) break;
-                if constexpr (kPair) umma_commit_pair_at(smem_u32(&S->acc_full[buf]), first);
-                else umma_commit(&S->acc_full[buf]);
+                if (elected) commit(&S->acc_full[buf]);
+                __syncwarp();
             }
-            if (dead) mm_raise(S, MXK_DEV_TIMEOUT_PIPE);
+            if (dead && elected) mm_raise(S, MXK_DEV_TIMEOUT_PIPE);
         }
     } else if (warp == 2 || warp == 3) {
         // -------------------------------------------------------- scale-tile builders
@@ -322,7 +357,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
             for (int i = 0; i < 4; ++i) v |= (kb + i < a.nkb ? (uint32_t)__ldg(p + kb + i) : 127u) << (8 * i);
             return v;
         };
-        constexpr int kXj = kPair ? 8 : 4;
+        constexpr int kXj = 4 * kXTiles;   // rows of an accumulator per lane
         uint32_t sfg = 0;
         bool dead = false;
         for (int t = unit; !dead && mm_tile<kPair>(a, start, before, t, tl); t += n_units) {
@@ -360,27 +395,26 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
             for (int i = i0; i < n_groups; i += 2) {
                 const uint32_t gg = sfg + (uint32_t)i, slot = gg % (uint32_t)a.sf_slots, par = (gg / (uint32_t)a.sf_slots) & 1u;
                 bool ok = true;
-                if (lane == 0) ok = wait_bar(&S->sf_empty[slot], par ^ 1u);
+                if (lane == 0) ok = mbar_wait(&S->sf_empty[slot], par ^ 1u, wait_ns, abort_flag);
                 ok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;
                 if (!ok) { dead = true; break; }
-                uint4* dst = reinterpret_cast<uint4*>(sf_tiles + slot * kMmSfSlotBytes);
+                uint4* dst = reinterpret_cast<uint4*>(sf_tiles + slot * kSfSlotBytes);
                 dst[lane] = make_uint4(ww[0], ww[1], ww[2], ww[3]);
-                dst[32 + lane] = make_uint4(wx[0], wx[1], wx[2], wx[3]);
-                if constexpr (kPair) dst[64 + lane] = make_uint4(wx[4], wx[5], wx[6], wx[7]);
+#pragma unroll
+                for (int j = 0; j < kXTiles; ++j) dst[32 * (j + 1) + lane] = make_uint4(wx[4 * j], wx[4 * j + 1], wx[4 * j + 2], wx[4 * j + 3]);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (i + 2 < n_groups) load_group(g_first + i + 2, wx, ww);   // in flight while the copy is issued and the slot awaited
                 if (lane == 0) {
-                    const uint32_t tsf = tmem_base + (uint32_t)a.sf_col + slot * (uint32_t)a.sf_slot_cols;
+                    const uint32_t tsf = tmem_base + (uint32_t)a.sf_col + slot * kSfSlotCols;
                     const uint64_t sfdesc = umma_smem_desc_sf(smem_u32(dst));
                     if constexpr (kPair) {
                         if (leader) {   // one copy serves both CTAs: the partner's tile must be in place
                             ok = wait_bar(&S->sf_peer[slot], par);
                             if (ok) {
                                 tc_fence_after();
-                                utccp_32x128b_warpx4_pair(tsf, sfdesc);
-                                utccp_32x128b_warpx4_pair(tsf + 4, sfdesc + (kMmSfTile >> 4));
-                                utccp_32x128b_warpx4_pair(tsf + 8, sfdesc + (2 * kMmSfTile >> 4));
+#pragma unroll
+                                for (int j = 0; j < kSfTiles; ++j) utccp_32x128b_warpx4_pair(tsf + 4 * j, sfdesc + (j * kMmSfTile >> 4));
                                 umma_commit_pair(mapa_u32(smem_u32(&S->sf_full[slot]), first));
                             }
                         } else {
@@ -388,8 +422,8 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                         }
                     } else {
                         tc_fence_after();
-                        utccp_32x128b_warpx4(tsf, sfdesc);
-                        utccp_32x128b_warpx4(tsf + 4, sfdesc + (kMmSfTile >> 4));
+#pragma unroll
+                        for (int j = 0; j < kSfTiles; ++j) utccp_32x128b_warpx4(tsf + 4 * j, sfdesc + (j * kMmSfTile >> 4));
                         umma_commit(&S->sf_full[slot]);
                     }
                 }
@@ -402,8 +436,11 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
     } else {
         // ------------------------------------------------------------------- epilogue
         // Warp (q, part) reads TMEM lanes 32q .. 32q+31 (its output columns) and every second chunk of
-        // 16 accumulator columns (rows of x).
+        // 16 accumulator columns (rows of x).  The accumulators are drained into registers, rounded to bf16 on the
+        // way, and given back before anything is stored.
         const int q = warp & 3, part = (warp - kMmFirstEpi) >> 2;
+        // neighbouring lanes swap halves of a row pair, so that a lane stores two columns at once
+        const bool twos = ((a.out_stride | (long long)(reinterpret_cast<uintptr_t>(a.out) >> 1)) & 1) == 0;
         uint32_t it = 0;
         bool dead = false;
         for (int t = unit; mm_tile<kPair>(a, start, before, t, tl); t += n_units, ++it) {
@@ -416,35 +453,65 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
             ok = __all_sync(0xFFFFFFFFu, ok ? 1 : 0) != 0;
             if (!ok) { dead = true; break; }
             tc_fence_after();
-            const uint32_t tacc = tmem_base + buf * (uint32_t)a.acc_stride + ((uint32_t)(q * 32) << 16);
             const int n_chunks = tl.bt >> 4;
             const int col = tl.w_row + 128 * (int)half + q * 32 + lane;
-            const bool col_ok = col < a.cols;
-            uint16_t* out = a.out + (long long)tl.x_row * a.out_stride + col;
-            for (int c = part; c < n_chunks; c += 4) {
+            const uint32_t tacc = tmem_base + buf * (uint32_t)a.bt_max + ((uint32_t)(q * 32) << 16);
+            uint32_t pk[kMmChunks][8];   // two rows of this lane's column per register
+#pragma unroll
+            for (int u = 0; u < kMmChunks; u += 2) {
                 uint32_t v[2][16];
-                const bool two = c + 2 < n_chunks;
-                tmem_ld16(tacc + c * 16, v[0]);
+                const int c = part + 2 * u;
+                const bool two = u + 1 < kMmChunks && c + 2 < n_chunks;
+                if (c < n_chunks) tmem_ld16(tacc + c * 16, v[0]);
                 if (two) tmem_ld16(tacc + (c + 2) * 16, v[1]);
                 tmem_wait_ld();
+                if (a.splits > 1) {
+                    if (c < n_chunks) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    if (u == 1 && !two) break;
-                    const int r0 = (c + 2 * u) * 16;
-                    if (a.splits > 1) {
+                        for (int j = 0; j < 16; ++j) red[(c * 16 + j) * 128 + q * 32 + lane] = __uint_as_float(v[0][j]);
+                    }
+                    if (two) {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) red[(r0 + j) * 128 + q * 32 + lane] = __uint_as_float(v[u][j]);
-                    } else {
+                        for (int j = 0; j < 16; ++j) red[((c + 2) * 16 + j) * 128 + q * 32 + lane] = __uint_as_float(v[1][j]);
+                    }
+                } else {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (col_ok && r0 + j < tl.valid)
-                                out[(long long)(r0 + j) * a.out_stride] = __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(v[u][j])));
+                    for (int j = 0; j < 8; ++j) {
+                        pk[u][j] = pack_bf16x2(__uint_as_float(v[0][2 * j]), __uint_as_float(v[0][2 * j + 1]));
+                        if (u + 1 < kMmChunks) pk[u + 1][j] = pack_bf16x2(__uint_as_float(v[1][2 * j]), __uint_as_float(v[1][2 * j + 1]));
                     }
                 }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) arrive_leader(&S->acc_empty[buf]);
+            if (a.splits == 1) {
+#pragma unroll
+                for (int u = 0; u < kMmChunks; ++u) {
+                    const int c = part + 2 * u, r0 = c * 16;
+                    if (c >= n_chunks || r0 >= tl.valid) break;
+                    if (twos) {
+                        uint16_t* out = a.out + (long long)(tl.x_row + r0 + (lane & 1)) * a.out_stride + (col & ~1);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const uint32_t mine = pk[u][j], other = __shfl_xor_sync(0xFFFFFFFFu, mine, 1);
+                            const uint32_t v = (lane & 1) ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
+                            if (r0 + 2 * j + (lane & 1) < tl.valid) {
+                                if ((col | 1) < a.cols) *reinterpret_cast<uint32_t*>(out) = v;
+                                else if ((col & ~1) < a.cols) *out = (uint16_t)v;
+                            }
+                            out += 2 * a.out_stride;
+                        }
+                    } else if (col < a.cols) {
+                        uint16_t* out = a.out + (long long)(tl.x_row + r0) * a.out_stride + col;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            if (r0 + j < tl.valid) *out = (uint16_t)(pk[u][j >> 1] >> (16 * (j & 1)));
+                            out += a.out_stride;
+                        }
+                    }
+                }
+            }
             if (a.splits > 1) {
                 // every split's partial tile is in its own shared memory; split s adds up rows s, s + splits, ...
                 const uint32_t peer_step = ctas;
@@ -496,11 +563,13 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
     }
 }
 
+// one CTA per tile of 128 weight rows: few rows of x, the weights' stream is all that counts
 __global__ void __launch_bounds__(kMmThreads, 1)
 k_matmul(const MmArgs a, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w) {
-    mm_body<false>(a, &tm_x, &tm_w);
+    mm_body<false, kMmStageKb>(a, &tm_x, &tm_w);
 }
+// a CTA pair per tile of 256 weight rows (2-CTA MMA)
 __global__ void __launch_bounds__(kMmThreads, 1)
 k_matmul_pair(const MmArgs a, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w) {
-    mm_body<true>(a, &tm_x, &tm_w);
+    mm_body<true, kMmPairStageKb>(a, &tm_x, &tm_w);
 }

@@ -273,42 +273,34 @@ int mxk_fp8_matmul(const MxkMatmulArgs* p, void* stream) {
     const bool pair = mean > 128 && cols > 128;
     const int groups = (a.nkb + 3) / 4;
     a.splits = 1;
+    a.n_tiles = (a.cols + (pair ? 255 : 127)) / (pair ? 256 : 128);
     if (pair) {
-        a.n_tiles = (a.cols + 255) / 256;
-        a.bt_max = 240;
-        if (!p->offsets) {
-            // extent of a tile along x: the one whose last wave wastes least
-            double best = 1e30;
-            for (int bt = 240; bt >= 64; bt -= 16) {
-                const int64_t tt = (rows + bt - 1) / bt;
-                const int64_t real = ((rows + tt - 1) / tt + 15) / 16 * 16;
-                const int64_t waves = (tt * a.n_tiles + kSms / 2 - 1) / (kSms / 2);
-                const double cost = (double)waves * ((double)std::max<int64_t>(real, 96) + 8.0);
-                if (cost < best) { best = cost; a.bt_max = bt; }
-            }
+        double best = 1e30;
+        for (int bt = kMmRowsMax; bt >= 64; bt -= 16) {
+            const int64_t tt = (mean + bt - 1) / bt, real = ((mean + tt - 1) / tt + 15) / 16 * 16;
+            const int64_t waves = (experts * tt * a.n_tiles + kSms / 2 - 1) / (kSms / 2);
+            const double cost = (double)waves * (130.0 + real);
+            if (cost < best) { best = cost; a.bt_max = bt; }
         }
-        a.box = a.bt_max / 2;
     } else {
-        a.n_tiles = (a.cols + 127) / 128;
         a.bt_max = mean <= 32 ? (int)std::min<int64_t>(32, (mean + 15) / 16 * 16) : 128;
         if (p->offsets) a.bt_max = mean <= 16 ? 32 : 128;
-        a.box = a.bt_max;
         const int64_t tiles = (p->offsets ? std::min<int64_t>(experts, rows) : (rows + a.bt_max - 1) / a.bt_max) * a.n_tiles;
         while (a.splits < 8 && tiles * a.splits * 2 <= kSms && a.splits * 2 <= groups) a.splits *= 2;
     }
-    a.acc_stride = a.bt_max;
-    a.sf_slot_cols = pair ? 12 : 8;
-    a.sf_col = 2 * a.acc_stride;
-    a.sf_slots = std::min(kMmMaxSfSlots, (kMmTmemCols - a.sf_col) / a.sf_slot_cols);
-    const int stage = kMmWBytes + a.box * 128;
-    const int fixed = 1024 + a.sf_slots * kMmSfSlotBytes + (a.splits > 1 ? a.bt_max * 512 : 0) + (int)sizeof(MmSmem) + 2 * (a.experts + 1) * 4;
+    a.box = pair ? a.bt_max / 2 : a.bt_max;
+    const int sf_tiles = pair ? 3 : 2;
+    a.sf_col = 2 * a.bt_max;
+    a.sf_slots = std::min(kMmMaxSfSlots, (kMmTmemCols - a.sf_col) / (4 * sf_tiles));
+    const int stage = (pair ? kMmPairStageKb : kMmStageKb) * (kMmWBytes + a.box * 128);
+    const int fixed = 1024 + a.sf_slots * sf_tiles * kMmSfTile + (a.splits > 1 ? a.bt_max * 512 : 0) + (int)sizeof(MmSmem) + 2 * (a.experts + 1) * 4;
     a.n_stages = std::min(kMmMaxStages, (kMmSmemLimit - fixed) / stage);
     const int smem = fixed + a.n_stages * stage;
     CUtensorMap tm_x, tm_w;
     if (int rc = byte_map(&tm_x, p->x, rows, depth, p->x_stride, a.box)) return rc;
     if (int rc = byte_map(&tm_w, p->w, experts * cols, depth, p->w_stride, 128)) return rc;
-    const void* fn = pair ? (const void*)k_matmul_pair : (const void*)k_matmul;
-    if (int rc = allow_smem(fn, pair ? 1 : 2, kMmSmemLimit)) return rc;
+    const auto fn = pair ? k_matmul_pair : k_matmul;
+    if (int rc = allow_smem((const void*)fn, pair ? 1 : 2, kMmSmemLimit)) return rc;
     const int cluster = (pair ? 2 : 1) * a.splits;
     const int64_t tiles_most = ((p->offsets ? std::min<int64_t>(experts, rows) : 0) + (rows + a.bt_max - 1) / a.bt_max) * a.n_tiles;
     if (tiles_most > (1 << 30)) return fail(MXK_ERR_BAD_ARG, "fp8_matmul: more than 2^30 tiles");
@@ -322,7 +314,7 @@ int mxk_fp8_matmul(const MxkMatmulArgs* p, void* stream) {
     at.id = cudaLaunchAttributeClusterDimension;
     at.val.clusterDim.x = cluster; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
     cfg.attrs = &at; cfg.numAttrs = cluster > 1 ? 1 : 0;
-    const cudaError_t e = pair ? cudaLaunchKernelEx(&cfg, k_matmul_pair, a, tm_x, tm_w) : cudaLaunchKernelEx(&cfg, k_matmul, a, tm_x, tm_w);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, a, tm_x, tm_w);
     return e == cudaSuccess ? 0 : cuda_fail(e, "launch k_matmul");
 }
 
