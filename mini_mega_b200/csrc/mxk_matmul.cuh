@@ -57,9 +57,10 @@ struct MmArgs {
     int n_tiles;               // weight tiles of a group
     int bt_max, box;           // rows of x per tile at most; rows per TMA box (pairs: half of them)
     int n_stages, sf_slots, sf_col;
-    int splits;                // CTAs (pairs) of a cluster that share a tile's K extent
+    int splits;                // CTAs (pairs) of a cluster that share a tile's K extent: 1, 2, 4 or 8
     int w_sf_rows, w_per_row;  // rows of a group's weight scale plane; 1: one scale row per weight row
     int zero_tail;             // clear out rows behind the last group
+    FastDiv fbt, fnt;          // division by bt_max and n_tiles
     uint32_t formats;          // operand format bits of the instruction descriptor
     unsigned long long wait_ns;
 };
@@ -72,6 +73,14 @@ struct MmSmem {
     uint32_t tmem_base;
     int abort_flag;
 };
+
+// the barriers of MmSmem lie behind one another; what each expects
+constexpr int kMmBarriers = 2 * kMmMaxStages + 3 * kMmMaxSfSlots + 6;
+__device__ __forceinline__ uint32_t mm_barrier_count(int i, uint32_t ctas, uint32_t splits) {
+    const int k = i - (2 * kMmMaxStages + 3 * kMmMaxSfSlots);
+    return k < 2 ? 1u : k < 4 ? kMmEpiWarps * ctas : kMmEpiWarps * splits;   // copies and commits; acc_empty; red_full, red_free
+}
+static_assert(offsetof(MmSmem, tmem_base) == kMmBarriers * sizeof(uint64_t), "barriers first, without gaps");
 
 struct MmTile {
     int group, w_row, x_row, bt, valid;    // w_row: first weight row inside the group; x_row, bt: rows of x
@@ -90,11 +99,16 @@ __device__ __forceinline__ bool mm_tile(const MmArgs& a, const int* start, const
         const int mid = (lo + hi) >> 1;
         if (before[mid] <= t) lo = mid; else hi = mid;
     }
-    const int n = start[lo + 1] - start[lo], tt = (n + a.bt_max - 1) / a.bt_max, i = t - before[lo];
-    const bool rows_fast = n <= a.cols;
-    const int xt = rows_fast ? i % tt : i / a.n_tiles, wt = rows_fast ? i / tt : i % a.n_tiles;
+    const int n = start[lo + 1] - start[lo], i = t - before[lo];
+    int xt = 0, wt = i, per = n;
+    if (n > a.bt_max) {
+        const int tt = a.fbt.div(n + a.bt_max - 1);
+        if (n <= a.cols) { wt = i / tt; xt = i - wt * tt; }
+        else { xt = a.fnt.div(i); wt = i - xt * a.n_tiles; }
+        per = (n + tt - 1) / tt;
+    }
     o.group = lo;
-    o.bt = ((n + tt - 1) / tt + 15) & ~15;   // the group's rows spread evenly over its tiles
+    o.bt = (per + 15) & ~15;   // the group's rows spread evenly over its tiles
     o.w_row = wt * (kPair ? 256 : 128);
     o.x_row = start[lo] + xt * o.bt;
     o.valid = min(o.bt, n - xt * o.bt);
@@ -115,11 +129,11 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
     asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
@@ -158,58 +172,71 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
     volatile int* abort_flag = &S->abort_flag;
     const uint64_t wait_ns = a.wait_ns;
 
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < kMmMaxStages; ++s) { mbar_init(&S->full[s], 1); mbar_init(&S->empty[s], 1); }
-        for (int s = 0; s < kMmMaxSfSlots; ++s) { mbar_init(&S->sf_full[s], 1); mbar_init(&S->sf_empty[s], 1); mbar_init(&S->sf_peer[s], 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(&S->acc_full[s], 1); mbar_init(&S->acc_empty[s], kMmEpiWarps * ctas); }
-        mbar_init(&S->red_full, kMmEpiWarps * a.splits);
-        mbar_init(&S->red_free, kMmEpiWarps * a.splits);
-        S->abort_flag = 0;
+    // Start-up, kept short because it is a fifth of a small product: warp 0 initialises the barriers, builds the
+    // group table and goes on to its first loads without waiting for the others; warp 1 meanwhile allocates TMEM.
+    if (clustered && warp != 0) cluster_arrive();
+    if (warp == 0) {
+        if (lane == 0) {
+            tma_prefetch_desc(tm_w);
+            tma_prefetch_desc(tm_x);
+        }
+        for (int i = lane; i < kMmBarriers; i += 32) mbar_init(&S->full[0] + i, mm_barrier_count(i, ctas, (uint32_t)a.splits));
+        if (lane == 0) S->abort_flag = 0;
         mbar_fence_init();
         fence_proxy_async_smem();
-        tma_prefetch_desc(tm_x);
-        tma_prefetch_desc(tm_w);
-    }
-    if (warp == 1) {
-        if constexpr (kPair) { tmem_alloc_pair(&S->tmem_base, kMmTmemCols); tmem_relinquish_pair(); }
-        else { tmem_alloc(&S->tmem_base, kMmTmemCols); tmem_relinquish(); }
-    }
-    // Group table.  Offsets come from the device and are not trusted: clamped into [0, rows] and made
-    // ascending (a running maximum), groups are disjoint whatever they held and no tile reaches outside.
-    for (int e = threadIdx.x; e <= a.experts; e += kMmThreads)
-        start[e] = a.offsets ? min(max(a.offsets[e], 0), a.rows) : e * a.rows;
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 0) {   // running maximum of the offsets, then the exclusive sum of the groups' tile counts
-        int run = 0;
-        for (int e0 = 0; e0 <= a.experts; e0 += 32) {
-            const int e = e0 + lane;
-            int m = e <= a.experts ? start[e] : 0;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) m = max(m, __shfl_up_sync(0xFFFFFFFFu, m, d));   // lanes below d get their own value
-            m = max(m, run);
-            if (e <= a.experts) start[e] = m;
-            run = __shfl_sync(0xFFFFFFFFu, m, 31);
+        if (clustered) {
+            __syncwarp();
+            cluster_arrive();
         }
-        __syncwarp();
-        run = 0;
-        for (int e0 = 0; e0 < a.experts; e0 += 32) {
-            const int e = e0 + lane;
-            const int v = e < a.experts ? ((start[e + 1] - start[e] + a.bt_max - 1) / a.bt_max) * a.n_tiles : 0;
-            int s = v;
+        // Group table.  Offsets come from the device and are not trusted: clamped into [0, rows] and made
+        // ascending (a running maximum), groups are disjoint whatever they held and no tile reaches outside.
+        if (!a.offsets) {
+            if (lane == 0) {
+                start[0] = before[0] = 0;
+                start[1] = a.rows;
+                before[1] = a.fbt.div(a.rows + a.bt_max - 1) * a.n_tiles;
+            }
+        } else {
+#pragma unroll 4
+            for (int e = lane; e <= a.experts; e += 32) start[e] = min(max(a.offsets[e], 0), a.rows);
+            __syncwarp();
+            // every lane walks a contiguous share of the groups; the shares are joined by warp scans
+            const int share = a.experts / 32 + 1, e0 = lane * share, e1 = min(e0 + share, a.experts + 1);
+            int top = 0;
+            for (int e = e0; e < e1; ++e) start[e] = top = max(top, start[e]);
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) top = max(top, __shfl_up_sync(0xFFFFFFFFu, top, d));   // lanes below d get their own value
+            int below = __shfl_up_sync(0xFFFFFFFFu, top, 1);
+            if (lane == 0) below = 0;
+            for (int e = e0; e < e1; ++e) start[e] = max(below, start[e]);
+            __syncwarp();
+            int sum = 0;
+            for (int e = e0; e < e1; ++e) {
+                before[e] = sum;
+                if (e < a.experts) sum += a.fbt.div(start[e + 1] - start[e] + a.bt_max - 1) * a.n_tiles;
+            }
+            const int own = sum;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
-                const int o = __shfl_up_sync(0xFFFFFFFFu, s, d);
-                if (lane >= d) s += o;
+                const int o = __shfl_up_sync(0xFFFFFFFFu, sum, d);
+                if (lane >= d) sum += o;
             }
-            if (e < a.experts) before[e] = run + s - v;
-            run += __shfl_sync(0xFFFFFFFFu, s, 31);
+            for (int e = e0; e < e1; ++e) before[e] += sum - own;
         }
-        if (lane == 0) before[a.experts] = run;
+        __syncwarp();
+        asm volatile("barrier.cta.arrive 1, %0;" ::"n"(kMmThreads) : "memory");
+    } else {
+        if (warp == 1) {
+            if constexpr (kPair) { tmem_alloc_pair(&S->tmem_base, kMmTmemCols); tmem_relinquish_pair(); }
+            else { tmem_alloc(&S->tmem_base, kMmTmemCols); tmem_relinquish(); }
+        }
+        tc_fence_before();
+        asm volatile("barrier.cta.sync 1, %0;" ::"n"(kMmThreads) : "memory");
+        tc_fence_after();
     }
-    if (clustered) cluster_sync_all(); else __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem_base = *(volatile uint32_t*)&S->tmem_base;
+    // the partner's barriers must exist before anything arrives on them; a split's producer has no partner
+    if (kPair || (clustered && warp != 0)) cluster_wait();
+    const uint32_t tmem_base = warp == 0 ? 0u : *(volatile uint32_t*)&S->tmem_base;
 
     const int unit = (int)blockIdx.x / (int)(ctas * a.splits), n_units = (int)gridDim.x / (int)(ctas * a.splits);
     // K blocks of this split, cut at multiples of four blocks (one scale word holds four)
@@ -226,6 +253,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
         else mbar_arrive(bar);
     };
     MmTile tl;
+    bool left = false;   // this thread has arrived at the closing cluster barrier
 
     if (warp == 0) {
         // --------------------------------------------------------------- TMA producer
@@ -448,7 +476,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
             bool ok = true;
             if (lane == 0) ok = wait_bar(&S->acc_full[buf], use & 1u);
             ok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;
-            // the previous tile's partials have been read by every split before they are overwritten
+            // every split has added up the previous tile's partials before they are overwritten
             if (ok && a.splits > 1 && it > 0) ok = mbar_wait_cluster(&S->red_free, (it - 1) & 1u, wait_ns, abort_flag);
             ok = __all_sync(0xFFFFFFFFu, ok ? 1 : 0) != 0;
             if (!ok) { dead = true; break; }
@@ -457,24 +485,34 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
             const int col = tl.w_row + 128 * (int)half + q * 32 + lane;
             const uint32_t tacc = tmem_base + buf * (uint32_t)a.bt_max + ((uint32_t)(q * 32) << 16);
             uint32_t pk[kMmChunks][8];   // two rows of this lane's column per register
-#pragma unroll
-            for (int u = 0; u < kMmChunks; u += 2) {
-                uint32_t v[2][16];
-                const int c = part + 2 * u;
-                const bool two = u + 1 < kMmChunks && c + 2 < n_chunks;
-                if (c < n_chunks) tmem_ld16(tacc + c * 16, v[0]);
-                if (two) tmem_ld16(tacc + (c + 2) * 16, v[1]);
+            // split K: row r of the tile is added up by split r % splits, into whose shared memory every split writes
+            // its partial row, [split][r / splits][128]
+            const int log_splits = __ffs(a.splits) - 1, own_rows = a.bt_max >> log_splits;
+            auto push = [&](int c) {
+                uint32_t v[16];
+                tmem_ld16(tacc + c * 16, v);
                 tmem_wait_ld();
-                if (a.splits > 1) {
-                    if (c < n_chunks) {
+                const uint32_t at = smem_u32(red + split * own_rows * 128 + q * 32 + lane);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) red[(c * 16 + j) * 128 + q * 32 + lane] = __uint_as_float(v[0][j]);
-                    }
-                    if (two) {
+                for (int j = 0; j < 16; ++j) {
+                    const int r = c * 16 + j;
+                    if (r >= tl.valid) break;
+                    st_cluster_f32(mapa_u32(at + (uint32_t)(r >> log_splits) * 512u, (uint32_t)(r & (a.splits - 1)) * ctas + half), v[j]);
+                }
+            };
+            if (a.splits > 1) {
+#pragma unroll 1
+                for (int c = part; c < n_chunks; c += 2) push(c);
+            } else {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) red[((c + 2) * 16 + j) * 128 + q * 32 + lane] = __uint_as_float(v[1][j]);
-                    }
-                } else {
+                for (int u = 0; u < kMmChunks; u += 2) {
+                    uint32_t v[2][16];
+                    const int c = part + 2 * u;
+                    const bool two = u + 1 < kMmChunks && c + 2 < n_chunks;
+                    if (c >= n_chunks) break;
+                    tmem_ld16(tacc + c * 16, v[0]);
+                    if (two) tmem_ld16(tacc + (c + 2) * 16, v[1]);
+                    tmem_wait_ld();
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         pk[u][j] = pack_bf16x2(__uint_as_float(v[0][2 * j]), __uint_as_float(v[0][2 * j + 1]));
@@ -513,19 +551,18 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                 }
             }
             if (a.splits > 1) {
-                // every split's partial tile is in its own shared memory; split s adds up rows s, s + splits, ...
-                const uint32_t peer_step = ctas;
-                if (lane == 0)
-                    for (int s = 0; s < a.splits; ++s) mbar_arrive_cluster(mapa_u32(smem_u32(&S->red_full), (uint32_t)s * peer_step + half));
+                if (lane < a.splits) mbar_arrive_cluster(mapa_u32(smem_u32(&S->red_full), (uint32_t)lane * ctas + half));
                 ok = mbar_wait_cluster(&S->red_full, it & 1u, wait_ns, abort_flag);
                 ok = __all_sync(0xFFFFFFFFu, ok ? 1 : 0) != 0;
                 if (!ok) { dead = true; break; }
+                const bool more = t + n_units < before[a.experts];
+                if (!more) { cluster_arrive(); left = true; }   // nothing of this CTA touches another one's memory from here on
                 const int c0 = tl.w_row + 128 * (int)half + lane * 4;
                 for (int r = split + a.splits * (warp - kMmFirstEpi); r < tl.valid; r += a.splits * kMmEpiWarps) {
-                    const uint32_t at = smem_u32(red + r * 128 + lane * 4);
-                    float4 sum = ld_cluster_f4(mapa_u32(at, half));
+                    const float4* part_row = reinterpret_cast<const float4*>(red + (r >> log_splits) * 128) + lane;
+                    float4 sum = part_row[0];
                     for (int s = 1; s < a.splits; ++s) {
-                        const float4 o = ld_cluster_f4(mapa_u32(at, (uint32_t)s * peer_step + half));
+                        const float4 o = part_row[s * own_rows * 32];
                         sum.x += o.x; sum.y += o.y; sum.z += o.z; sum.w += o.w;
                     }
                     uint16_t* dst = a.out + (long long)(tl.x_row + r) * a.out_stride + c0;
@@ -539,9 +576,10 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                         if (c0 + 3 < a.cols) dst[3] = (uint16_t)(hi >> 16);
                     }
                 }
-                __syncwarp();
-                if (lane == 0)
-                    for (int s = 0; s < a.splits; ++s) mbar_arrive_cluster(mapa_u32(smem_u32(&S->red_free), (uint32_t)s * peer_step + half));
+                if (more) {
+                    __syncwarp();
+                    if (lane < a.splits) mbar_arrive_cluster(mapa_u32(smem_u32(&S->red_free), (uint32_t)lane * ctas + half));
+                }
             }
         }
         if (dead && lane == 0) mm_raise(S, MXK_DEV_TIMEOUT_PIPE);
@@ -554,9 +592,15 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
             }
         }
     }
-    // nobody leaves while the partner may still signal or read this CTA's shared memory
+    // nobody leaves while a partner may still signal or write this CTA's shared memory
     tc_fence_before();
-    if (clustered) cluster_sync_all(); else __syncthreads();
+    if (clustered) {
+        __syncwarp();
+        if (!kPair && warp == 0) cluster_wait();   // the arrival at the start is still open
+        if (!left) cluster_arrive();
+        cluster_wait();
+    }
+    __syncthreads();
     tc_fence_after();
     if (warp == 1) {
         if constexpr (kPair) tmem_dealloc_pair(tmem_base, kMmTmemCols); else tmem_dealloc(tmem_base, kMmTmemCols);

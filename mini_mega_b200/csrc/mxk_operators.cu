@@ -9,6 +9,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <string>
 
@@ -127,6 +128,43 @@ int unsort_grad_launch(const UnsortGradArgs& a, int vec, int grid, int threads, 
             if constexpr (kType != kTypeFp32) k_unsort_grad<kType, 2><<<grid, threads, 0, st>>>(a);
     }
     return launched("launch k_unsort_grad");
+}
+
+// How a product is cut: CTA pairs or single CTAs, rows of x per tile, CTAs that share a tile's K extent.  The cut
+// with the least estimated time, from the parts that were measured on a B200 (us; K blocks of 128):
+//   start, tile hand-over and end     single 6.2, pair 8.5, and 0.018 per row of x in a tile
+//   one K block of a tile             single (16 KB + 128 B x rows) at 140 GB/s per SM (512 x 4096 x 7168, 128-row
+//                                     tiles: 20.7 us), pair 145 ns + 0.6 ns x rows (128: 230, 192: 267, 224: 279 ns)
+//   partial sums between splits       1.2 + 0.014 x rows
+// Both sides, measured: 1 x 4096 x 6144 1 / 2 / 4 splits 13.0 / 10.5 / 9.5 us; 128 x 2048 x 6144 tiles of 128 rows in 4
+// splits 12.0, of 64 rows 11.1; 512 x 4096 x 7168 single 20.7, pairs 23.8; 2048 x 4096 x 7168 single 59.8, pairs 55.4;
+// 1 x 2048 x 6144 in 8 splits 14.3 against 8.8 in 4: few clusters of eight fit the GPU at once.
+struct MmShape { bool pair; int bt, splits; };
+MmShape mm_shape(int64_t rows, int64_t cols, int nkb, int64_t experts, bool grouped) {
+    double mean = (double)rows / (double)experts;
+    if (grouped) mean += 2.0 * std::sqrt(mean);   // groups differ in size: room for most of them in one tile
+    const int64_t n = std::max<int64_t>(1, (int64_t)std::ceil(mean)), groups = std::min(experts, rows);
+    MmShape best{false, 16, 1};
+    double least = 1e30;
+    auto offer = [&](bool pair, int bt, int splits, int64_t units) {
+        const int64_t tt = (n + bt - 1) / bt, real = ((n + tt - 1) / tt + 15) / 16 * 16;
+        const int64_t tiles = groups * tt * ((cols + (pair ? 255 : 127)) / (pair ? 256 : 128)), waves = (tiles + units - 1) / units;
+        const double block = pair ? 0.145 + 0.0006 * real : (16384.0 + 128.0 * bt) / 140e3;
+        const double time = (pair ? 8.5 : 6.2) + 0.018 * real + (double)waves * (double)((nkb + splits - 1) / splits) * block +
+                            (splits > 1 ? 1.2 + 0.014 * real : 0.0);
+        if (time < least) { least = time; best = MmShape{pair, bt, splits}; }
+    };
+    const int k_groups = (nkb + 3) / 4;
+    for (int bt : {16, 32, 48, 64, 96, 128}) {
+        if (bt > 16 && bt >= n + 32) break;
+        offer(false, bt, 1, kSms);
+        if (k_groups >= 2) offer(false, bt, 2, 72);
+        if (k_groups >= 4) offer(false, bt, 4, 34);
+        if (k_groups >= 8) offer(false, bt, 8, 8);
+    }
+    if (cols > 128)
+        for (int bt = 64; bt <= kMmRowsMax && bt < n + 32; bt += 16) offer(true, bt, 1, kSms / 2);
+    return best;
 }
 
 int dtype_bytes(int dtype) { return dtype == MXK_DTYPE_FP32 ? 4 : 2; }
@@ -269,26 +307,14 @@ int mxk_fp8_matmul(const MxkMatmulArgs* p, void* stream) {
     a.formats = ((uint32_t)p->w_format << 7) | ((uint32_t)p->x_format << 10);   // w is the MMA's A operand, x its B
     a.wait_ns = p->max_spins > 0 ? (unsigned long long)p->max_spins * 250ull : 2000000000ull;
 
-    const int64_t mean = (rows + experts - 1) / experts;   // rows of a group, on average
-    const bool pair = mean > 128 && cols > 128;
-    const int groups = (a.nkb + 3) / 4;
-    a.splits = 1;
+    const MmShape sh = mm_shape(rows, cols, a.nkb, experts, p->offsets != nullptr);
+    const bool pair = sh.pair;
+    a.bt_max = sh.bt;
+    a.splits = sh.splits;
     a.n_tiles = (a.cols + (pair ? 255 : 127)) / (pair ? 256 : 128);
-    if (pair) {
-        double best = 1e30;
-        for (int bt = kMmRowsMax; bt >= 64; bt -= 16) {
-            const int64_t tt = (mean + bt - 1) / bt, real = ((mean + tt - 1) / tt + 15) / 16 * 16;
-            const int64_t waves = (experts * tt * a.n_tiles + kSms / 2 - 1) / (kSms / 2);
-            const double cost = (double)waves * (130.0 + real);
-            if (cost < best) { best = cost; a.bt_max = bt; }
-        }
-    } else {
-        a.bt_max = mean <= 32 ? (int)std::min<int64_t>(32, (mean + 15) / 16 * 16) : 128;
-        if (p->offsets) a.bt_max = mean <= 16 ? 32 : 128;
-        const int64_t tiles = (p->offsets ? std::min<int64_t>(experts, rows) : (rows + a.bt_max - 1) / a.bt_max) * a.n_tiles;
-        while (a.splits < 8 && tiles * a.splits * 2 <= kSms && a.splits * 2 <= groups) a.splits *= 2;
-    }
     a.box = pair ? a.bt_max / 2 : a.bt_max;
+    a.fbt = FastDiv::make((uint32_t)a.bt_max);
+    a.fnt = FastDiv::make((uint32_t)a.n_tiles);
     const int sf_tiles = pair ? 3 : 2;
     a.sf_col = 2 * a.bt_max;
     a.sf_slots = std::min(kMmMaxSfSlots, (kMmTmemCols - a.sf_col) / (4 * sf_tiles));
