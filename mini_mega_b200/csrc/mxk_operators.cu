@@ -57,6 +57,29 @@ int allow_smem(const void* fn, int slot, int bytes) {
     return 0;
 }
 
+// Whether a cluster of 16 plan CTAs can run on the current device (more than the portable 8: asked once).
+bool sixteen_fit(int smem) {
+    static thread_local uint64_t asked = 0, fits = 0;   // bit = device
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return false;
+    if (!((asked >> dev) & 1)) {
+        cudaLaunchConfig_t cfg;
+        std::memset(&cfg, 0, sizeof(cfg));
+        cfg.gridDim = dim3(16, 1, 1); cfg.blockDim = dim3(kPlanThreads, 1, 1); cfg.dynamicSmemBytes = (size_t)smem;
+        cudaLaunchAttribute at;
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = 16; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+        cfg.attrs = &at; cfg.numAttrs = 1;
+        int n = 0;
+        const bool ok = cudaFuncSetAttribute((const void*)k_plan, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                        cudaOccupancyMaxActiveClusters(&n, k_plan, &cfg) == cudaSuccess && n >= 1;
+        if (!ok) (void)cudaGetLastError();
+        if (ok) fits |= 1ull << dev;
+        asked |= 1ull << dev;
+    }
+    return (fits >> dev) & 1;
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -83,52 +106,61 @@ int byte_map(CUtensorMap* m, const void* base, int64_t rows, int64_t k, int64_t 
     return r == CUDA_SUCCESS ? 0 : fail(MXK_ERR_TENSOR_MAP, "cuTensorMapEncodeTiled failed, CUresult " + std::to_string((int)r));
 }
 
-// Work split of the row kernels: `span` whole rows per CTA of narrow rows, column parts of one row
-// when rows are wide or few.
-struct RowGrid { int span, vecs, part_vecs, threads; dim3 grid; };
-RowGrid row_grid(int tokens, int row_bytes, int vec, int per_cta) {
-    RowGrid g;
-    g.vecs = row_bytes / vec;
-    g.span = std::max(1, per_cta / g.vecs);
-    g.part_vecs = g.vecs;
-    if (g.span == 1) {
-        const int parts_min = (g.vecs + per_cta - 1) / per_cta;
-        const int parts_fill = std::min((g.vecs + 63) / 64, (2 * kSms + tokens - 1) / tokens);   // few tokens: more CTAs per row
-        const int parts = std::min(65535, std::max(parts_min, parts_fill));
-        g.part_vecs = (g.vecs + parts - 1) / parts;
-    } else {
-        g.span = std::max(1, std::min(g.span, (tokens + 2 * kSms - 1) / (2 * kSms)));
-    }
-    const int work = g.span * g.part_vecs;
-    g.threads = std::min(256, std::max(64, (work + 31) / 32 * 32));
-    g.grid = dim3((unsigned)((tokens + g.span - 1) / g.span), (unsigned)((g.vecs + g.part_vecs - 1) / g.part_vecs), 1);
-    return g;
+// Tile of the row kernels: column parts of at most 256 threads x u vectors, as many tokens beside one another
+// as fit the CTA; with few tokens, more and narrower parts, so that every SM has some.
+dim3 row_frame(RowFrame& f, int tokens, int topk, int row_bytes, int vec, int u, const int32_t* row_of_pair) {
+    f.row_of_pair = row_of_pair;
+    f.tokens = tokens; f.topk = topk; f.pairs = tokens * topk; f.row_bytes = row_bytes;
+    f.vecs = row_bytes / vec;
+    const int most = kRowThreads * u;
+    int parts = (f.vecs + most - 1) / most;
+    if ((int64_t)tokens * parts < 2 * kSms) parts = std::min<int64_t>((f.vecs + 32 * u - 1) / (32 * u), (2 * kSms + tokens - 1) / tokens);
+    parts = std::min(std::max(parts, (f.vecs + most - 1) / most), 65535);
+    // a part is `wide` threads x u vectors; rows so wide that 65535 parts do not cover them are refused by the callers
+    f.wide = (f.vecs + parts * u - 1) / (parts * u);
+    f.part_vecs = f.wide * u;
+    parts = (f.vecs + f.part_vecs - 1) / f.part_vecs;
+    f.tall = std::max(1, std::min(kRowThreads / f.wide, kRowBatch / topk));
+    f.tall = (int)std::min<int64_t>(f.tall, std::max<int64_t>(1, (tokens * (int64_t)parts + 2 * kSms - 1) / (2 * kSms)));
+    f.batch = std::max(1, kRowBatch / (f.tall * topk));
+    f.fwide = FastDiv::make((uint32_t)f.wide); f.ftopk = FastDiv::make((uint32_t)topk);
+    const int64_t columns = (tokens + f.tall - 1) / f.tall, resident = std::max<int64_t>(1, kSms * 8 / parts);
+    const int grid = (int)std::min(columns, resident);
+    f.batch = (int)std::min<int64_t>(f.batch, (columns + grid - 1) / grid);
+    return dim3((unsigned)grid, (unsigned)parts, 1);
 }
+constexpr int kMaxRowBytes = 1 << 24;
 
 int bad_tables(int64_t tokens, int topk) { return tokens < 0 || topk < 1 || topk > 256 || tokens * topk > (1 << 30); }
 
 template <int kType>
-int unsort_launch(const UnsortArgs& a, int vec, const RowGrid& g, cudaStream_t st) {
+int unsort_launch(const UnsortArgs& a, int vec, dim3 grid, cudaStream_t st) {
     switch (vec) {
-        case 16: k_unsort_rows<kType, 16><<<g.grid, g.threads, 0, st>>>(a); break;
-        case 8: k_unsort_rows<kType, 8><<<g.grid, g.threads, 0, st>>>(a); break;
-        case 4: k_unsort_rows<kType, 4><<<g.grid, g.threads, 0, st>>>(a); break;
+        case 16: k_unsort_rows<kType, 16, 1><<<grid, kRowThreads, 0, st>>>(a); break;
+        case 8: k_unsort_rows<kType, 8, 2><<<grid, kRowThreads, 0, st>>>(a); break;
+        case 4: k_unsort_rows<kType, 4, 4><<<grid, kRowThreads, 0, st>>>(a); break;
         default:
-            if constexpr (kType != kTypeFp32) k_unsort_rows<kType, 2><<<g.grid, g.threads, 0, st>>>(a);
+            if constexpr (kType != kTypeFp32) k_unsort_rows<kType, 2, 4><<<grid, kRowThreads, 0, st>>>(a);
     }
     return launched("launch k_unsort_rows");
 }
-template <int kType>
-int unsort_grad_launch(const UnsortGradArgs& a, int vec, int grid, int threads, cudaStream_t st) {
-    switch (vec) {
-        case 16: k_unsort_grad<kType, 16><<<grid, threads, 0, st>>>(a); break;
-        case 8: k_unsort_grad<kType, 8><<<grid, threads, 0, st>>>(a); break;
-        case 4: k_unsort_grad<kType, 4><<<grid, threads, 0, st>>>(a); break;
-        default:
-            if constexpr (kType != kTypeFp32) k_unsort_grad<kType, 2><<<grid, threads, 0, st>>>(a);
-    }
+template <int kType, int V>
+int unsort_grad_vec(const UnsortGradArgs& a, int grid, cudaStream_t st) {
+    if (a.drows && a.dw) k_unsort_grad<kType, V, true, true><<<grid, kRowThreads, 0, st>>>(a);
+    else if (a.drows) k_unsort_grad<kType, V, true, false><<<grid, kRowThreads, 0, st>>>(a);
+    else k_unsort_grad<kType, V, false, true><<<grid, kRowThreads, 0, st>>>(a);
     return launched("launch k_unsort_grad");
 }
+template <int kType>
+int unsort_grad_launch(const UnsortGradArgs& a, int vec, int grid, cudaStream_t st) {
+    switch (vec) {
+        case 16: return unsort_grad_vec<kType, 16>(a, grid, st);
+        case 8: return unsort_grad_vec<kType, 8>(a, grid, st);
+        case 4: return unsort_grad_vec<kType, 4>(a, grid, st);
+        default: return unsort_grad_vec<kType, kType == kTypeFp32 ? 4 : 2>(a, grid, st);
+    }
+}
+int unroll_of(int vec) { return vec >= 16 ? 1 : vec == 8 ? 2 : 4; }
 
 // How a product is cut: CTA pairs or single CTAs, rows of x per tile, CTAs that share a tile's K extent.  The cut
 // with the least estimated time, from the parts that were measured on a B200 (us; K blocks of 128):
@@ -186,15 +218,21 @@ int mxk_plan_tokens(const void* topk_idx, int32_t idx_bytes, int64_t idx_stride,
     a.pairs = tokens * topk; a.topk = topk; a.first = first_expert; a.experts = num_experts;
     a.ftopk = FastDiv::make((uint32_t)topk);
     a.row_of_pair = row_of_pair; a.pair_of_row = pair_of_row; a.offsets = offsets;
-    const int ctas = a.pairs > kPlanThreads * kPlanKeep ? kPlanClusterMax : 1;
-    a.per_warp = ((a.pairs + ctas * kPlanWarps - 1) / (ctas * kPlanWarps) + 31) / 32 * 32;
-    if (a.per_warp == 0) a.per_warp = 32;
-    a.per_cta = a.per_warp * kPlanWarps;
-    if (int rc = allow_smem((const void*)k_plan, 0, (kPlanWarps + 1) * kRowsMaxExperts * 4)) return rc;
+    while ((1 << a.bits) <= num_experts) ++a.bits;
+    const int smem_most = (kPlanWarps + 2) * plan_stride(kRowsMaxExperts) * 4;
+    if (int rc = allow_smem((const void*)k_plan, 0, smem_most)) return rc;
+    int ctas = 1, threads = std::max(256, (num_experts + 255) / 256 * 256);
+    if (a.pairs > 8 * 32 * kPlanKeep) {
+        threads = kPlanThreads;
+        ctas = a.pairs > 16384 && sixteen_fit(smem_most) ? 16 : 8;
+    }
+    const int warps = threads / 32;
+    a.per_warp = std::max(32, ((a.pairs + ctas * warps - 1) / (ctas * warps) + 31) / 32 * 32);
+    a.per_cta = a.per_warp * warps;
     cudaLaunchConfig_t cfg;
     std::memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3(ctas, 1, 1); cfg.blockDim = dim3(kPlanThreads, 1, 1);
-    cfg.dynamicSmemBytes = (size_t)(kPlanWarps + 1) * num_experts * 4;
+    cfg.gridDim = dim3(ctas, 1, 1); cfg.blockDim = dim3(threads, 1, 1);
+    cfg.dynamicSmemBytes = (size_t)(warps + 2) * plan_stride(num_experts) * 4;
     cfg.stream = static_cast<cudaStream_t>(stream);
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeClusterDimension;
@@ -207,7 +245,7 @@ int mxk_plan_tokens(const void* topk_idx, int32_t idx_bytes, int64_t idx_stride,
 int mxk_sort_tokens(const void* x, int64_t x_stride, int64_t row_bytes, const void* x_sf, int64_t sf_stride, int64_t sf_bytes,
                     int32_t tokens, int32_t topk, int32_t num_experts, const int32_t* row_of_pair, const int32_t* offsets,
                     void* rows, void* rows_sf, void* stream) {
-    if (bad_tables(tokens, topk) || num_experts < 1 || num_experts > kRowsMaxExperts || row_bytes < 1 || row_bytes > (1 << 28) || (x_sf && (sf_bytes < 1 || sf_bytes > (1 << 24))))
+    if (bad_tables(tokens, topk) || num_experts < 1 || num_experts > kRowsMaxExperts || row_bytes < 1 || row_bytes > kMaxRowBytes || (x_sf && (sf_bytes < 1 || sf_bytes > (1 << 24))))
         return fail(MXK_ERR_BAD_ARG, "sort_tokens: sizes out of range");
     if (tokens == 0) return 0;
     if (!x || !rows || !row_of_pair || !offsets || (x_sf && !rows_sf)) return fail(MXK_ERR_BAD_ARG, "sort_tokens: pointers must be non-null");
@@ -216,52 +254,49 @@ int mxk_sort_tokens(const void* x, int64_t x_stride, int64_t row_bytes, const vo
     std::memset(&a, 0, sizeof(a));
     a.x = static_cast<const uint8_t*>(x); a.x_sf = static_cast<const uint8_t*>(x_sf);
     a.rows = static_cast<uint8_t*>(rows); a.rows_sf = static_cast<uint8_t*>(rows_sf);
-    a.row_of_pair = row_of_pair; a.end = offsets + num_experts;
-    a.x_stride = x_stride; a.sf_stride = sf_stride; a.row_bytes = (int)row_bytes; a.sf_bytes = (int)sf_bytes;
+    a.end = offsets + num_experts;
+    a.x_stride = x_stride; a.sf_stride = sf_stride; a.sf_bytes = (int)sf_bytes;
     if (x_sf) {
         const int v = common_vec(addr(x_sf) | addr(rows_sf) | (uint64_t)sf_stride | (uint64_t)sf_bytes);
         a.sf_vec = v == 2 ? 1 : v;
     }
-    const RowGrid g = row_grid(tokens, a.row_bytes, vec, 1024);
-    a.tokens = tokens; a.topk = topk; a.pairs = tokens * topk; a.span = g.span; a.vecs = g.vecs; a.part_vecs = g.part_vecs;
-    a.fvecs = FastDiv::make((uint32_t)g.vecs);
+    const dim3 grid = row_frame(a.f, tokens, topk, (int)row_bytes, vec, unroll_of(vec), row_of_pair);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (vec) {
-        case 16: k_sort_rows<16><<<g.grid, g.threads, 0, st>>>(a); break;
-        case 8: k_sort_rows<8><<<g.grid, g.threads, 0, st>>>(a); break;
-        case 4: k_sort_rows<4><<<g.grid, g.threads, 0, st>>>(a); break;
-        case 2: k_sort_rows<2><<<g.grid, g.threads, 0, st>>>(a); break;
-        default: k_sort_rows<1><<<g.grid, g.threads, 0, st>>>(a); break;
+        case 16: k_sort_rows<16, 1><<<grid, kRowThreads, 0, st>>>(a); break;
+        case 8: k_sort_rows<8, 2><<<grid, kRowThreads, 0, st>>>(a); break;
+        case 4: k_sort_rows<4, 4><<<grid, kRowThreads, 0, st>>>(a); break;
+        case 2: k_sort_rows<2, 4><<<grid, kRowThreads, 0, st>>>(a); break;
+        default: k_sort_rows<1, 4><<<grid, kRowThreads, 0, st>>>(a); break;
     }
     return launched("launch k_sort_rows");
 }
 
 int mxk_unsort_tokens(const void* rows, int32_t dtype, int64_t rows_stride, const float* weights, int64_t weights_stride,
                       int32_t tokens, int32_t topk, int32_t hidden, const int32_t* row_of_pair, void* y, void* stream) {
-    if (bad_tables(tokens, topk) || hidden < 1 || hidden > (1 << 26) || dtype < MXK_DTYPE_BF16 || dtype > MXK_DTYPE_FP32)
+    if (bad_tables(tokens, topk) || hidden < 1 || hidden > kMaxRowBytes / 4 || dtype < MXK_DTYPE_BF16 || dtype > MXK_DTYPE_FP32)
         return fail(MXK_ERR_BAD_ARG, "unsort_tokens: sizes or type out of range");
     if (tokens == 0) return 0;
     if (!rows || !row_of_pair || !y) return fail(MXK_ERR_BAD_ARG, "unsort_tokens: pointers must be non-null");
     UnsortArgs a;
     std::memset(&a, 0, sizeof(a));
-    a.rows = static_cast<const uint8_t*>(rows); a.w = weights; a.y = static_cast<uint8_t*>(y); a.row_of_pair = row_of_pair;
-    a.rows_stride = rows_stride; a.w_stride = weights_stride; a.row_bytes = hidden * dtype_bytes(dtype);
-    const int vec = common_vec(addr(rows) | addr(y) | (uint64_t)rows_stride | (uint64_t)a.row_bytes);
+    a.rows = static_cast<const uint8_t*>(rows); a.w = weights; a.y = static_cast<uint8_t*>(y);
+    a.rows_stride = rows_stride; a.w_stride = weights_stride;
+    const int row_bytes = hidden * dtype_bytes(dtype);
+    const int vec = common_vec(addr(rows) | addr(y) | (uint64_t)rows_stride | (uint64_t)row_bytes);
     if (vec < dtype_bytes(dtype)) return fail(MXK_ERR_BAD_ARG, "unsort_tokens: rows and y must be aligned to their element type");
-    const RowGrid g = row_grid(tokens, a.row_bytes, vec, 256);
-    a.tokens = tokens; a.topk = topk; a.pairs = tokens * topk; a.span = g.span; a.vecs = g.vecs; a.part_vecs = g.part_vecs;
-    a.fvecs = FastDiv::make((uint32_t)g.vecs);
+    const dim3 grid = row_frame(a.f, tokens, topk, row_bytes, vec, unroll_of(vec), row_of_pair);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == MXK_DTYPE_BF16) return unsort_launch<kTypeBf16>(a, vec, g, st);
-    if (dtype == MXK_DTYPE_FP16) return unsort_launch<kTypeFp16>(a, vec, g, st);
-    return unsort_launch<kTypeFp32>(a, vec, g, st);
+    if (dtype == MXK_DTYPE_BF16) return unsort_launch<kTypeBf16>(a, vec, grid, st);
+    if (dtype == MXK_DTYPE_FP16) return unsort_launch<kTypeFp16>(a, vec, grid, st);
+    return unsort_launch<kTypeFp32>(a, vec, grid, st);
 }
 
 int mxk_unsort_tokens_grad(const void* dy, int64_t dy_stride, const void* rows, int64_t rows_stride, int32_t dtype,
                            const float* weights, int64_t weights_stride, int32_t tokens, int32_t topk, int32_t num_experts,
                            int32_t hidden, const int32_t* row_of_pair, const int32_t* offsets, void* drows, float* dweights,
                            void* stream) {
-    if (bad_tables(tokens, topk) || num_experts < 1 || num_experts > kRowsMaxExperts || hidden < 1 || hidden > (1 << 26) || dtype < MXK_DTYPE_BF16 || dtype > MXK_DTYPE_FP32)
+    if (bad_tables(tokens, topk) || num_experts < 1 || num_experts > kRowsMaxExperts || hidden < 1 || hidden > kMaxRowBytes / 4 || dtype < MXK_DTYPE_BF16 || dtype > MXK_DTYPE_FP32)
         return fail(MXK_ERR_BAD_ARG, "unsort_tokens_grad: sizes or type out of range");
     if (tokens == 0 || (!drows && !dweights)) return 0;
     if (!dy || !weights || !row_of_pair || !offsets || (dweights && !rows)) return fail(MXK_ERR_BAD_ARG, "unsort_tokens_grad: pointers must be non-null");
@@ -277,11 +312,13 @@ int mxk_unsort_tokens_grad(const void* dy, int64_t dy_stride, const void* rows, 
     const int vec = common_vec(bits);
     if (vec < dtype_bytes(dtype)) return fail(MXK_ERR_BAD_ARG, "unsort_tokens_grad: tensors must be aligned to their element type");
     a.vecs = a.row_bytes / vec;
-    const int threads = std::min(256, std::max(32, (a.vecs + 31) / 32 * 32));
+    a.team = 1;   // warps per token: as many as the row has columns for
+    while (a.team < 8 && a.vecs > 32 * a.team) a.team *= 2;
+    const int grid = (int)(((int64_t)tokens * a.team + 7) / 8);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == MXK_DTYPE_BF16) return unsort_grad_launch<kTypeBf16>(a, vec, tokens, threads, st);
-    if (dtype == MXK_DTYPE_FP16) return unsort_grad_launch<kTypeFp16>(a, vec, tokens, threads, st);
-    return unsort_grad_launch<kTypeFp32>(a, vec, tokens, threads, st);
+    if (dtype == MXK_DTYPE_BF16) return unsort_grad_launch<kTypeBf16>(a, vec, grid, st);
+    if (dtype == MXK_DTYPE_FP16) return unsort_grad_launch<kTypeFp16>(a, vec, grid, st);
+    return unsort_grad_launch<kTypeFp32>(a, vec, grid, st);
 }
 
 int mxk_fp8_matmul(const MxkMatmulArgs* p, void* stream) {

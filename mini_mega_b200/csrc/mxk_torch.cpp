@@ -31,7 +31,7 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 typedef std::optional<Tensor> MaybeTensor;
 
-constexpr int64_t kMaxExperts = 1024, kMaxTopk = 256, kMaxRows = int64_t(1) << 30;
+constexpr int64_t kMaxExperts = 1024, kMaxTopk = 256, kMaxRows = int64_t(1) << 30, kMaxHidden = int64_t(1) << 22;
 
 template <class E, class... A>
 [[noreturn]] void raise(const A&... parts) {
@@ -208,10 +208,10 @@ py::object sort_tokens(const Tensor& x, const Tensor& row_of_pair, const Tensor&
     const char* fn = "sort_tokens_by_expert";
     check_plan(fn, row_of_pair, pair_of_row, offsets);
     MXK_TYPE(type_code(x.scalar_type()) >= 0 || byte_type(x.scalar_type()), fn, ": x must be a bf16, fp16, fp32 or 8-bit tensor");
-    MXK_VALUE(x.dim() == 2 && x.size(0) == row_of_pair.size(0) && x.size(1) >= 1 && x.size(1) <= (1 << 26), fn, ": x must be [", row_of_pair.size(0), ", hidden], got ", x.sizes());
+    MXK_VALUE(x.dim() == 2 && x.size(0) == row_of_pair.size(0) && x.size(1) >= 1 && x.size(1) <= kMaxHidden, fn, ": x must be [", row_of_pair.size(0), ", hidden], got ", x.sizes());
     if (x_sf) {
         MXK_TYPE(x_sf->scalar_type() == at::kByte && x.element_size() == 1, fn, ": x_sf are uint8 exponents of 8-bit rows");
-        MXK_VALUE(x_sf->dim() == 2 && x_sf->size(0) == x.size(0) && x_sf->size(1) >= 1 && x_sf->size(1) <= (1 << 24), fn, ": x_sf must be [", x.size(0), ", hidden / 128], got ", x_sf->sizes());
+        MXK_VALUE(x_sf->dim() == 2 && x_sf->size(0) == x.size(0) && x_sf->size(1) >= 1 && x_sf->size(1) <= kMaxHidden, fn, ": x_sf must be [", x.size(0), ", hidden / 128], got ", x_sf->sizes());
     }
     same_device(fn, x, {&row_of_pair, &pair_of_row, &offsets, x_sf ? &*x_sf : nullptr});
     const bool grad = x.requires_grad() && at::GradMode::is_enabled();
@@ -230,7 +230,7 @@ Tensor unsort_tokens(const Tensor& rows, const Tensor& row_of_pair, const Tensor
     const char* fn = "unsort_tokens_by_expert";
     check_plan(fn, row_of_pair, pair_of_row, offsets);
     MXK_TYPE(type_code(rows.scalar_type()) >= 0, fn, ": rows must be a bf16, fp16 or fp32 tensor");
-    MXK_VALUE(rows.dim() == 2 && rows.size(0) == row_of_pair.numel() && rows.size(1) >= 1 && rows.size(1) <= (1 << 26), fn, ": rows must be [", row_of_pair.numel(), ", hidden], got ", rows.sizes());
+    MXK_VALUE(rows.dim() == 2 && rows.size(0) == row_of_pair.numel() && rows.size(1) >= 1 && rows.size(1) <= kMaxHidden, fn, ": rows must be [", row_of_pair.numel(), ", hidden], got ", rows.sizes());
     const Tensor weights = topk_weights ? *topk_weights : Tensor();
     if (weights.defined()) {
         MXK_TYPE(weights.scalar_type() == at::kFloat, fn, ": topk_weights must be a float32 tensor");
