@@ -268,7 +268,9 @@ __device__ __forceinline__ void clear_row(uint8_t* row, int bytes) {
 
 // ---- sort: rows[row_of_pair[p]] = x[p / topk] -----------------------------------------------
 // A byte copy, so it serves every element type.  A vector of x is loaded once and stored to the token's topk rows:
-// memory sees tokens * row bytes in and pairs * row bytes out.  @SORT@
+// memory sees tokens * row bytes in and pairs * row bytes out.
+// 4096 tokens x 8, 7168 bytes: 48 us = 5.5 TB/s; bulk copies from shared memory, wider CTAs or streaming stores ran
+// within 3 % of it, a plain fill of the same bytes (no scatter, no reads) at 6.6 TB/s.
 struct SortArgs {
     RowFrame f;
     const uint8_t* x;
@@ -342,7 +344,8 @@ __global__ void __launch_bounds__(kRowThreads) k_sort_rows(const SortArgs a) {
 
 // ---- unsort: y[t] = sum_j w[t, j] rows[row_of_pair[t, j]] ------------------------------------
 // j ascending, FP32, one rounding at the end.  A thread has its vectors of up to eight of the token's rows in
-// flight; memory sees pairs * row bytes in, tokens * row bytes out.  @UNSORT@
+// flight; memory sees pairs * row bytes in, tokens * row bytes out.
+// 4096 tokens x 8, 7168 bf16: 90 us = 5.9 TB/s (249 us with the rows' numbers loaded in front of every vector).
 struct UnsortArgs {
     RowFrame f;
     const uint8_t* rows;
@@ -409,7 +412,9 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_unsort_rows(const UnsortArgs
 // ---- gradient of the weighted unsort -----------------------------------------------------------
 // drows[row(t, j)] = w[t, j] dy[t];  dw[t, j] = <dy[t], rows[row(t, j)]>.  A team of 1, 2, 4 or 8 warps (by the row's
 // width) takes one token.  dy is read once per eight pairs, the eight rows' vectors are requested together; a dot is
-// summed per lane, over the warp, over the team, always in that order.  @GRAD@
+// summed per lane, over the warp, over the team, always in that order.
+// 2048 tokens x 8, 6144 bf16: 69 us = 6.2 TB/s; with the loads one after the other 92 us, and with the 64 registers that
+// four CTAs per SM leave (spills) 120 us: two CTAs with everything in registers keep enough bytes in flight.
 struct UnsortGradArgs {
     const uint8_t* dy;
     const uint8_t* rows;       // needed for dw only
