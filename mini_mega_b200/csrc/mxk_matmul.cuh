@@ -41,7 +41,6 @@ constexpr int kMmMaxSfSlots = 8;
 constexpr int kMmSfTile = 512;                 // 128 rows x 4 scale bytes
 constexpr int kMmStageKb = 2, kMmPairStageKb = 2;   // K blocks of a ring stage
 constexpr int kMmRowsMax = 224;                // columns of an accumulator: 2 x 224 leave 64 TMEM columns to the scales
-constexpr int kMmChunks = kMmRowsMax / 16 / 2;  // 16-column chunks a warp drains of one accumulator
 constexpr int kMmWBytes = 128 * 128;           // weight tile of one K block
 constexpr int kMmMaxExperts = 1024;
 constexpr int kMmTmemCols = 512;
@@ -154,7 +153,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
     const uint32_t x_bytes = (uint32_t)a.box * 128u;
     const uint32_t stage_bytes = (uint32_t)kStageKb * ((uint32_t)kMmWBytes + x_bytes);   // [w]..[x].., tiles of 128-byte rows
     uint8_t* sf_tiles = tiles + (size_t)a.n_stages * stage_bytes;
-    float* red = reinterpret_cast<float*>(sf_tiles + a.sf_slots * kSfSlotBytes);   // [bt_max][128], splits > 1 only
+    float* red = reinterpret_cast<float*>(sf_tiles + a.sf_slots * kSfSlotBytes);   // [bt_max][128] partial sums, splits > 1 only
     MmSmem* S = reinterpret_cast<MmSmem*>(reinterpret_cast<uint8_t*>(red) + (a.splits > 1 ? (size_t)a.bt_max * 512 : 0));
     int* start = reinterpret_cast<int*>(S + 1);
     int* before = start + a.experts + 1;  // both [experts + 1]
@@ -462,11 +461,12 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
     } else {
         // ------------------------------------------------------------------- epilogue
         // Warp (q, part) reads TMEM lanes 32q .. 32q+31 (its output columns) and every second chunk of
-        // 16 accumulator columns (rows of x).  The accumulators are drained into registers, rounded to bf16 on the
-        // way, and given back before anything is stored.
+        // 16 accumulator columns (rows of x), and stores each row's 32 columns as one 64-byte piece straight from
+        // registers.  Shared memory is the busy resource while the MMAs run (their operand reads and the TMA writes
+        // use its bandwidth up), so turning the tile round there to store 16 bytes a lane, or by shuffles to store 4,
+        // is slower although it stores less often: 4096 x 4096 x 1024 25.4 us like this, 27.6 through shared
+        // memory, 32.0 with shuffles (rows off every alignment, 4095 columns: 28.0, 40.6, 29.0).
         const int q = warp & 3, part = (warp - kMmFirstEpi) >> 2;
-        // neighbouring lanes swap halves of a row pair, so that a lane stores two columns at once
-        const bool twos = ((a.out_stride | (long long)(reinterpret_cast<uintptr_t>(a.out) >> 1)) & 1) == 0;
         uint32_t it = 0;
         bool dead = false;
         for (int t = unit; mm_tile<kPair>(a, start, before, t, tl); t += n_units, ++it) {
@@ -480,9 +480,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
             if (!ok) { dead = true; break; }
             tc_fence_after();
             const int n_chunks = tl.bt >> 4;
-            const int col = tl.w_row + 128 * (int)half + q * 32 + lane;
             const uint32_t tacc = tmem_base + buf * (uint32_t)a.bt_max + ((uint32_t)(q * 32) << 16);
-            uint32_t pk[kMmChunks][8];   // two rows of this lane's column per register
             // split K: row r of the tile is added up by split r % splits, into whose shared memory every split writes
             // its partial row, [split][r / splits][128]
             const int log_splits = __ffs(a.splits) - 1, own_rows = a.bt_max >> log_splits;
@@ -501,52 +499,33 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
             if (a.splits > 1) {
 #pragma unroll 1
                 for (int c = part; c < n_chunks; c += 2) push(c);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_leader(&S->acc_empty[buf]);
             } else {
+                const int col = tl.w_row + 128 * (int)half + q * 32 + lane;
+                uint32_t v[16];
+                if (part < n_chunks) tmem_ld16(tacc + part * 16, v);
+                tmem_wait_ld();
+#pragma unroll 1
+                for (int c = part; c < n_chunks; c += 2) {
+                    uint32_t pk[8];
 #pragma unroll
-                for (int u = 0; u < kMmChunks; u += 2) {
-                    uint32_t v[2][16];
-                    const int c = part + 2 * u;
-                    const bool two = u + 1 < kMmChunks && c + 2 < n_chunks;
-                    if (c >= n_chunks) break;
-                    tmem_ld16(tacc + c * 16, v[0]);
-                    if (two) tmem_ld16(tacc + (c + 2) * 16, v[1]);
-                    tmem_wait_ld();
+                    for (int j = 0; j < 8; ++j) pk[j] = pack_bf16x2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                    const bool more = c + 2 < n_chunks;
+                    if (more) tmem_ld16(tacc + (c + 2) * 16, v);   // in flight while this chunk is stored
+                    uint16_t* dst = a.out + (long long)(tl.x_row + c * 16) * a.out_stride + col;
+                    const int n_rows = col < a.cols ? tl.valid - c * 16 : 0;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        pk[u][j] = pack_bf16x2(__uint_as_float(v[0][2 * j]), __uint_as_float(v[0][2 * j + 1]));
-                        if (u + 1 < kMmChunks) pk[u + 1][j] = pack_bf16x2(__uint_as_float(v[1][2 * j]), __uint_as_float(v[1][2 * j + 1]));
+                    for (int j = 0; j < 16; ++j) {
+                        if (j < n_rows) *dst = (uint16_t)(pk[j >> 1] >> (16 * (j & 1)));
+                        dst += a.out_stride;
                     }
+                    if (more) tmem_wait_ld();
                 }
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_leader(&S->acc_empty[buf]);
-            if (a.splits == 1) {
-#pragma unroll
-                for (int u = 0; u < kMmChunks; ++u) {
-                    const int c = part + 2 * u, r0 = c * 16;
-                    if (c >= n_chunks || r0 >= tl.valid) break;
-                    if (twos) {
-                        uint16_t* out = a.out + (long long)(tl.x_row + r0 + (lane & 1)) * a.out_stride + (col & ~1);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const uint32_t mine = pk[u][j], other = __shfl_xor_sync(0xFFFFFFFFu, mine, 1);
-                            const uint32_t v = (lane & 1) ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
-                            if (r0 + 2 * j + (lane & 1) < tl.valid) {
-                                if ((col | 1) < a.cols) *reinterpret_cast<uint32_t*>(out) = v;
-                                else if ((col & ~1) < a.cols) *out = (uint16_t)v;
-                            }
-                            out += 2 * a.out_stride;
-                        }
-                    } else if (col < a.cols) {
-                        uint16_t* out = a.out + (long long)(tl.x_row + r0) * a.out_stride + col;
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            if (r0 + j < tl.valid) *out = (uint16_t)(pk[u][j >> 1] >> (16 * (j & 1)));
-                            out += a.out_stride;
-                        }
-                    }
-                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_leader(&S->acc_empty[buf]);
             }
             if (a.splits > 1) {
                 if (lane < a.splits) mbar_arrive_cluster(mapa_u32(smem_u32(&S->red_full), (uint32_t)lane * ctas + half));

@@ -164,29 +164,38 @@ int unroll_of(int vec) { return vec >= 16 ? 1 : vec == 8 ? 2 : 4; }
 
 // How a product is cut: CTA pairs or single CTAs, rows of x per tile, CTAs that share a tile's K extent.  The cut
 // with the least estimated time, from the parts that were measured on a B200 (us; K blocks of 128):
-//   start, tile hand-over and end     single 6.2, pair 8.5, and 0.018 per row of x in a tile
-//   one K block of a tile             single (16 KB + 128 B x rows) at 140 GB/s per SM (512 x 4096 x 7168, 128-row
-//                                     tiles: 20.7 us), pair 145 ns + 0.6 ns x rows (128: 230, 192: 267, 224: 279 ns)
-//   partial sums between splits       1.2 + 0.014 x rows
-// Both sides, measured: 1 x 4096 x 6144 1 / 2 / 4 splits 13.0 / 10.5 / 9.5 us; 128 x 2048 x 6144 tiles of 128 rows in 4
-// splits 12.0, of 64 rows 11.1; 512 x 4096 x 7168 single 20.7, pairs 23.8; 2048 x 4096 x 7168 single 59.8, pairs 55.4;
-// 1 x 2048 x 6144 in 8 splits 14.3 against 8.8 in 4: few clusters of eight fit the GPU at once.
+//   start, tile hand-over and end     single 5.6 and 0.006 per row of x in a tile, pair 8.0
+//   one K block of a tile             single 153 ns + 0.64 ns x rows (32 rows: 173, 64: 195, 128: 234), pair 145 ns +
+//                                     0.6 ns x rows (128 rows: 230, 192: 267, 224: 279)
+//   partial sums between splits       1.0 + 0.25 x splits + 0.012 x rows
+// and, beside them, the operands' way from memory (6.3 TB/s) and, for every tile of rows after a group's first, its
+// weights' way from L2 once more (12 TB/s).  Both sides, measured: 1 x 4096 x 6144 in 1 / 2 / 4 splits 12.8 / 10.6 /
+// 9.6 us; 128 x 2048 x 6144 tiles of 128 rows in 4 splits 12.5, of 64 rows 11.5; 512 x 4096 x 7168 single 19.4, pairs
+// 22.3; 2048 x 4096 x 7168 single 58.7, pairs 53.8; 32 groups of 200 rows x 4096 x 7168 pairs with one tile a group
+// 195, with two 272, single CTAs with two 254.  Splits only while every tile runs at once: a second round costs 7 us
+// (20 groups of 40 rows x 1000 x 2992: 21 us without splits, 24 in two, 45 in four), and 8 of them only for a few
+// tiles, because few clusters of eight fit the GPU at once (1 x 2048 x 6144: 14.3 us, in four 8.8).
 struct MmShape { bool pair; int bt, splits; };
-MmShape mm_shape(int64_t rows, int64_t cols, int nkb, int64_t experts, bool grouped) {
+MmShape mm_shape(int64_t rows, int64_t cols, int64_t depth, int64_t experts, bool grouped) {
+    const int nkb = (int)((depth + 127) / 128), k_groups = (nkb + 3) / 4;
     double mean = (double)rows / (double)experts;
-    if (grouped) mean += 2.0 * std::sqrt(mean);   // groups differ in size: room for most of them in one tile
+    if (grouped) mean = std::max(48.0, mean + 1.5 * std::sqrt(mean));   // groups differ in size: most shall fit one tile
     const int64_t n = std::max<int64_t>(1, (int64_t)std::ceil(mean)), groups = std::min(experts, rows);
+    const double weights = (double)groups * (double)cols * (double)depth;
+    const double memory = (weights + (double)rows * (double)depth + 2.0 * (double)rows * (double)cols) / 6.3e6;
     MmShape best{false, 16, 1};
     double least = 1e30;
     auto offer = [&](bool pair, int bt, int splits, int64_t units) {
         const int64_t tt = (n + bt - 1) / bt, real = ((n + tt - 1) / tt + 15) / 16 * 16;
         const int64_t tiles = groups * tt * ((cols + (pair ? 255 : 127)) / (pair ? 256 : 128)), waves = (tiles + units - 1) / units;
-        const double block = pair ? 0.145 + 0.0006 * real : (16384.0 + 128.0 * bt) / 140e3;
-        const double time = (pair ? 8.5 : 6.2) + 0.018 * real + (double)waves * (double)((nkb + splits - 1) / splits) * block +
-                            (splits > 1 ? 1.2 + 0.014 * real : 0.0);
+        if (splits > 1 && (grouped ? tiles + tiles / 2 : tiles) > units) return;
+        const double block = pair ? 0.145 + 0.0006 * real : 0.153 + 0.00064 * bt;
+        const double compute = (double)waves * (double)((nkb + splits - 1) / splits) * block;
+        const double time = (pair ? 8.0 : 5.6 + 0.006 * real) + std::max(compute, grouped ? memory : 0.0) +
+                            (grouped ? (double)(tt - 1) * weights / 12e6 : 0.0) +
+                            (splits > 1 ? 1.0 + 0.25 * splits + 0.012 * real : 0.0);
         if (time < least) { least = time; best = MmShape{pair, bt, splits}; }
     };
-    const int k_groups = (nkb + 3) / 4;
     for (int bt : {16, 32, 48, 64, 96, 128}) {
         if (bt > 16 && bt >= n + 32) break;
         offer(false, bt, 1, kSms);
@@ -344,7 +353,7 @@ int mxk_fp8_matmul(const MxkMatmulArgs* p, void* stream) {
     a.formats = ((uint32_t)p->w_format << 7) | ((uint32_t)p->x_format << 10);   // w is the MMA's A operand, x its B
     a.wait_ns = p->max_spins > 0 ? (unsigned long long)p->max_spins * 250ull : 2000000000ull;
 
-    const MmShape sh = mm_shape(rows, cols, a.nkb, experts, p->offsets != nullptr);
+    const MmShape sh = mm_shape(rows, cols, depth, experts, p->offsets != nullptr);
     const bool pair = sh.pair;
     a.bt_max = sh.bt;
     a.splits = sh.splits;
