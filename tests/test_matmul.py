@@ -277,3 +277,48 @@ def test_captured_replayed_on_two_streams_and_without_rows():
     assert mm.fp8_matmul(empty, w[0]).shape == (0, 640)
     assert mm.fp8_grouped_matmul(empty, w, torch.zeros(7, dtype=torch.int32, device="cuda")).shape == (0, 640)
     assert mm.matmul_status() == 0
+
+
+@pytest.mark.gpu
+def test_results_behind_two_to_the_31_elements():
+    """Element offsets of the last output rows pass 32 bits: 270000 rows of 8192 columns."""
+    rows, cols = 270000, 8192
+    g = _gen(9)
+    x, w = _data(g, (rows, 16), E4, True), _data(g, (cols, 16), E4, True)
+    out = mm.fp8_matmul(x, w)
+    for at in (0, 131072, 262143, 262144, 269999):
+        assert torch.equal(out[at], (x[at].double() @ w.double().t()).to(torch.bfloat16))
+    offsets = torch.tensor([0, 5, 262150, rows], dtype=torch.int32, device="cuda")
+    w3 = _data(g, (3, cols, 16), E4, True)
+    mm.fp8_grouped_matmul(x, w3, offsets, out=out)
+    for at, e in ((4, 0), (5, 1), (262149, 1), (262150, 2), (269999, 2)):
+        assert torch.equal(out[at], (x[at].double() @ w3[e].double().t()).to(torch.bfloat16))
+
+
+@pytest.mark.gpu
+def test_many_experts_and_long_depth():
+    g = _gen(10)
+    counts = [(7 * e) % 5 for e in range(1024)]
+    rows = sum(counts)
+    x, w = _data(g, (rows, 144), E4, True), _data(g, (1024, 40, 144), E4, True)
+    offsets = torch.tensor([0] + counts, device="cuda").cumsum(0).int()
+    out = mm.fp8_grouped_matmul(x, w, offsets)
+    owner = torch.repeat_interleave(torch.arange(1024, device="cuda"), torch.tensor(counts, device="cuda"))
+    want = torch.einsum("rk,rnk->rn", x.double(), w.double()[owner])
+    assert torch.equal(out, want.to(torch.bfloat16))
+    # 65536 columns of depth: 1 and 300 rows
+    w = _data(g, (200, 65536), E4, True)
+    for n in (1, 300):
+        x = _data(g, (n, 65536), E4, True)
+        assert torch.equal(mm.fp8_matmul(x, w), (x.double() @ w.double().t()).to(torch.bfloat16))
+
+
+@pytest.mark.gpu
+def test_results_do_not_depend_on_timing():
+    """The same bits on every run, splits of the depth included."""
+    g = _gen(11)
+    for rows, cols, depth in ((1, 512, 7168), (33, 1024, 4096), (700, 640, 2064)):
+        x, w = _data(g, (rows, depth), E4, False), _data(g, (cols, depth), E4, False)
+        first = mm.fp8_matmul(x, w)
+        for _ in range(20):
+            assert torch.equal(mm.fp8_matmul(x, w), first)
