@@ -305,6 +305,13 @@ __device__ __forceinline__ void tma_load_2d_pair_hint(void* smem_dst, const CUte
         : "memory");
 }
 
+// ---- programmatic dependent launch ---------------------------------------------------
+// A kernel launched with the programmatic attribute may begin while its predecessor in the stream still
+// runs; everything before grid_wait() must keep to its own shared and tensor memory.  After grid_wait() the
+// predecessor has ended and its writes are visible, as behind an ordinary launch.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---- tcgen05 ------------------------------------------------------------------
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_holder, uint32_t ncols) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_holder)),

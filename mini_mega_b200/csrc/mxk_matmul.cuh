@@ -171,6 +171,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
 
     // Start-up, kept short because it is a fifth of a small product: warp 0 initialises the barriers, builds the
     // group table and goes on to its first loads without waiting for the others; warp 1 meanwhile allocates TMEM.
+    grid_let_next_begin();
     if (clustered && warp != 0) cluster_arrive();
     if (warp == 0) {
         if (lane == 0) {
@@ -187,6 +188,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
         }
         // Group table.  Offsets come from the device and are not trusted: clamped into [0, rows] and made
         // ascending (a running maximum), groups are disjoint whatever they held and no tile reaches outside.
+        grid_wait();   // the kernels before this one in the stream have ended: from here on memory is read
         if (!a.offsets) {
             if (lane == 0) {
                 start[0] = before[0] = 0;
@@ -227,6 +229,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
             if constexpr (kPair) { tmem_alloc_pair(&S->tmem_base, kMmTmemCols); tmem_relinquish_pair(); }
             else { tmem_alloc(&S->tmem_base, kMmTmemCols); tmem_relinquish(); }
         }
+        grid_wait();
         tc_fence_before();
         asm volatile("barrier.cta.sync 1, %0;" ::"n"(kMmThreads) : "memory");
         tc_fence_after();

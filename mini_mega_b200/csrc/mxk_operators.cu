@@ -30,10 +30,23 @@ constexpr int kSms = 148;
 
 int fail(int code, const std::string& msg) { return mxk_set_error(code, msg); }
 int cuda_fail(cudaError_t e, const char* what) { return mxk_set_error((int)e, std::string(what) + ": " + cudaGetErrorString(e)); }
-int launched(const char* what) {
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? 0 : cuda_fail(e, what);
+
+// Every launch allows its kernel to begin while the one before it in the stream ends (grid_wait in the kernels).
+template <class... K, class... A>
+cudaError_t launch(void (*kernel)(K...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st, const A&... args) {
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = grid; cfg.blockDim = dim3((unsigned)threads, 1, 1); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    std::memset(at, 0, sizeof(at));
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)cluster; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
+int launched(cudaError_t e, const char* what) { return e == cudaSuccess ? 0 : cuda_fail(e, what); }
 
 // Largest power of two up to 16 that divides every given address, stride and length (in bytes).
 int common_vec(uint64_t bits) {
@@ -135,21 +148,23 @@ int bad_tables(int64_t tokens, int topk) { return tokens < 0 || topk < 1 || topk
 
 template <int kType>
 int unsort_launch(const UnsortArgs& a, int vec, dim3 grid, cudaStream_t st) {
+    cudaError_t e = cudaSuccess;
     switch (vec) {
-        case 16: k_unsort_rows<kType, 16, 1><<<grid, kRowThreads, 0, st>>>(a); break;
-        case 8: k_unsort_rows<kType, 8, 2><<<grid, kRowThreads, 0, st>>>(a); break;
-        case 4: k_unsort_rows<kType, 4, 4><<<grid, kRowThreads, 0, st>>>(a); break;
+        case 16: e = launch(k_unsort_rows<kType, 16, 1>, grid, kRowThreads, 0, 1, st, a); break;
+        case 8: e = launch(k_unsort_rows<kType, 8, 2>, grid, kRowThreads, 0, 1, st, a); break;
+        case 4: e = launch(k_unsort_rows<kType, 4, 4>, grid, kRowThreads, 0, 1, st, a); break;
         default:
-            if constexpr (kType != kTypeFp32) k_unsort_rows<kType, 2, 4><<<grid, kRowThreads, 0, st>>>(a);
+            if constexpr (kType != kTypeFp32) e = launch(k_unsort_rows<kType, 2, 4>, grid, kRowThreads, 0, 1, st, a);
     }
-    return launched("launch k_unsort_rows");
+    return launched(e, "launch k_unsort_rows");
 }
 template <int kType, int V>
 int unsort_grad_vec(const UnsortGradArgs& a, int grid, cudaStream_t st) {
-    if (a.drows && a.dw) k_unsort_grad<kType, V, true, true><<<grid, kRowThreads, 0, st>>>(a);
-    else if (a.drows) k_unsort_grad<kType, V, true, false><<<grid, kRowThreads, 0, st>>>(a);
-    else k_unsort_grad<kType, V, false, true><<<grid, kRowThreads, 0, st>>>(a);
-    return launched("launch k_unsort_grad");
+    cudaError_t e = cudaSuccess;
+    if (a.drows && a.dw) e = launch(k_unsort_grad<kType, V, true, true>, grid, kRowThreads, 0, 1, st, a);
+    else if (a.drows) e = launch(k_unsort_grad<kType, V, true, false>, grid, kRowThreads, 0, 1, st, a);
+    else e = launch(k_unsort_grad<kType, V, false, true>, grid, kRowThreads, 0, 1, st, a);
+    return launched(e, "launch k_unsort_grad");
 }
 template <int kType>
 int unsort_grad_launch(const UnsortGradArgs& a, int vec, int grid, cudaStream_t st) {
@@ -238,17 +253,7 @@ int mxk_plan_tokens(const void* topk_idx, int32_t idx_bytes, int64_t idx_stride,
     const int warps = threads / 32;
     a.per_warp = std::max(32, ((a.pairs + ctas * warps - 1) / (ctas * warps) + 31) / 32 * 32);
     a.per_cta = a.per_warp * warps;
-    cudaLaunchConfig_t cfg;
-    std::memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3(ctas, 1, 1); cfg.blockDim = dim3(threads, 1, 1);
-    cfg.dynamicSmemBytes = (size_t)(warps + 2) * plan_stride(num_experts) * 4;
-    cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = ctas; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
-    cfg.attrs = &at; cfg.numAttrs = ctas > 1 ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, k_plan, a);
-    return e == cudaSuccess ? 0 : cuda_fail(e, "launch k_plan");
+    return launched(launch(k_plan, dim3(ctas, 1, 1), threads, (size_t)(warps + 2) * plan_stride(num_experts) * 4, ctas, static_cast<cudaStream_t>(stream), a), "launch k_plan");
 }
 
 int mxk_sort_tokens(const void* x, int64_t x_stride, int64_t row_bytes, const void* x_sf, int64_t sf_stride, int64_t sf_bytes,
@@ -271,14 +276,15 @@ int mxk_sort_tokens(const void* x, int64_t x_stride, int64_t row_bytes, const vo
     }
     const dim3 grid = row_frame(a.f, tokens, topk, (int)row_bytes, vec, unroll_of(vec), row_of_pair);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t e = cudaSuccess;
     switch (vec) {
-        case 16: k_sort_rows<16, 1><<<grid, kRowThreads, 0, st>>>(a); break;
-        case 8: k_sort_rows<8, 2><<<grid, kRowThreads, 0, st>>>(a); break;
-        case 4: k_sort_rows<4, 4><<<grid, kRowThreads, 0, st>>>(a); break;
-        case 2: k_sort_rows<2, 4><<<grid, kRowThreads, 0, st>>>(a); break;
-        default: k_sort_rows<1, 4><<<grid, kRowThreads, 0, st>>>(a); break;
+        case 16: e = launch(k_sort_rows<16, 1>, grid, kRowThreads, 0, 1, st, a); break;
+        case 8: e = launch(k_sort_rows<8, 2>, grid, kRowThreads, 0, 1, st, a); break;
+        case 4: e = launch(k_sort_rows<4, 4>, grid, kRowThreads, 0, 1, st, a); break;
+        case 2: e = launch(k_sort_rows<2, 4>, grid, kRowThreads, 0, 1, st, a); break;
+        default: e = launch(k_sort_rows<1, 4>, grid, kRowThreads, 0, 1, st, a); break;
     }
-    return launched("launch k_sort_rows");
+    return launched(e, "launch k_sort_rows");
 }
 
 int mxk_unsort_tokens(const void* rows, int32_t dtype, int64_t rows_stride, const float* weights, int64_t weights_stride,
@@ -376,18 +382,8 @@ int mxk_fp8_matmul(const MxkMatmulArgs* p, void* stream) {
     const int cluster = (pair ? 2 : 1) * a.splits;
     const int64_t tiles_most = ((p->offsets ? std::min<int64_t>(experts, rows) : 0) + (rows + a.bt_max - 1) / a.bt_max) * a.n_tiles;
     if (tiles_most > (1 << 30)) return fail(MXK_ERR_BAD_ARG, "fp8_matmul: more than 2^30 tiles");
-    cudaLaunchConfig_t cfg;
-    std::memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(tiles_most, kSms / cluster) * cluster), 1, 1);
-    cfg.blockDim = dim3(kMmThreads, 1, 1);
-    cfg.dynamicSmemBytes = (size_t)smem;
-    cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = cluster; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
-    cfg.attrs = &at; cfg.numAttrs = cluster > 1 ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, a, tm_x, tm_w);
-    return e == cudaSuccess ? 0 : cuda_fail(e, "launch k_matmul");
+    const dim3 grid((unsigned)(std::min<int64_t>(tiles_most, kSms / cluster) * cluster), 1, 1);
+    return launched(launch(fn, grid, kMmThreads, (size_t)smem, cluster, static_cast<cudaStream_t>(stream), a, tm_x, tm_w), "launch k_matmul");
 }
 
 int mxk_matmul_status(int32_t* out) {

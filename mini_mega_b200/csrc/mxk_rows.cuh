@@ -59,6 +59,8 @@ __device__ __forceinline__ unsigned plan_peers(int e, int bits) {   // lanes who
 __host__ __device__ constexpr int plan_stride(int experts) { return experts | 1; }
 
 __global__ void __launch_bounds__(kPlanThreads, 1) k_plan(const PlanArgs a) {
+    grid_let_next_begin();
+    grid_wait();
     extern __shared__ int plan_smem[];
     const int stride = plan_stride(a.experts);
     int* mine = plan_smem;                        // [experts] pairs of this CTA
@@ -300,6 +302,8 @@ __device__ __forceinline__ void copy_scales(const SortArgs& a, const int* s_row,
 
 template <int V, int U>
 __global__ void __launch_bounds__(kRowThreads) k_sort_rows(const SortArgs a) {
+    grid_let_next_begin();
+    grid_wait();
     typedef typename VecOf<V>::T T;
     __shared__ int s_row[kRowBatch];
     const RowFrame& f = a.f;
@@ -356,6 +360,8 @@ struct UnsortArgs {
 
 template <int kType, int V, int U>
 __global__ void __launch_bounds__(kRowThreads, 4) k_unsort_rows(const UnsortArgs a) {
+    grid_let_next_begin();
+    grid_wait();
     constexpr int kEl = elem_bytes<kType>(), kN = V / kEl;
     typedef typename VecOf<V>::T T;
     __shared__ int s_row[kRowBatch];
@@ -430,6 +436,8 @@ struct UnsortGradArgs {
 
 template <int kType, int V, bool kRows, bool kDots>
 __global__ void __launch_bounds__(kRowThreads, 2) k_unsort_grad(const UnsortGradArgs a) {
+    grid_let_next_begin();
+    grid_wait();
     constexpr int kEl = elem_bytes<kType>(), kN = V / kEl;
     typedef typename VecOf<V>::T T;
     __shared__ float s_dot[2][8][8];
