@@ -25,6 +25,11 @@
 // of one hides under the MMAs of the next.  (Both as the halves of one tile of 448 rows were slower, although a
 // quarter fewer bytes cross L2: MMAs that alternate between two accumulators ran at 75 % of the pipe.)
 //
+// What bounds it: many rows, the tensor pipe at the clock that the 1 kW cap leaves (4096 x 4096 x 7168: 97 us = 2.48
+// PFLOP/s in a burst, pipe 82 - 92 % busy at 1.55 - 1.6 GHz; 119 us in a loop of seconds); few rows, the weights'
+// stream (32 groups of 4 rows x 4096 x 6144: 121 us = 6.7 TB/s); the smallest calls, a chain of round trips of
+// some 5 us that starts under the predecessor's end (programmatic launch).
+//
 // Few tiles (small batches): the K extent is split over the CTAs of a cluster, the partial tiles
 // are exchanged through distributed shared memory and added in the order of the splits, so results
 // do not depend on timing.
@@ -465,10 +470,9 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
         // ------------------------------------------------------------------- epilogue
         // Warp (q, part) reads TMEM lanes 32q .. 32q+31 (its output columns) and every second chunk of
         // 16 accumulator columns (rows of x), and stores each row's 32 columns as one 64-byte piece straight from
-        // registers.  Shared memory is the busy resource while the MMAs run (their operand reads and the TMA writes
-        // use its bandwidth up), so turning the tile round there to store 16 bytes a lane, or by shuffles to store 4,
-        // is slower although it stores less often: 4096 x 4096 x 1024 25.4 us like this, 27.6 through shared
-        // memory, 32.0 with shuffles (rows off every alignment, 4095 columns: 28.0, 40.6, 29.0).
+        // registers.  Beside the running MMAs that was faster than fewer, wider stores: 4096 x 4096 x 1024
+        // 25.4 us like this, 27.6 with chunks turned round in shared memory and 16 bytes a lane, 32.0 with shuffles
+        // and 4 bytes (rows off every alignment, 4095 columns: 28.0, 40.6, 29.0).
         const int q = warp & 3, part = (warp - kMmFirstEpi) >> 2;
         uint32_t it = 0;
         bool dead = false;
