@@ -234,6 +234,7 @@ int mxk_plan_tokens(const void* topk_idx, int32_t idx_bytes, int64_t idx_stride,
                     int32_t* offsets, void* stream) {
     if (bad_tables(tokens, topk) || num_experts < 1 || num_experts > kRowsMaxExperts || first_expert < 0 || (idx_bytes != 4 && idx_bytes != 8))
         return fail(MXK_ERR_BAD_ARG, "plan_tokens: need tokens * topk <= 2^30, 1 <= topk <= 256, 1 <= num_experts <= 1024, ids of 4 or 8 bytes");
+    if (idx_stride < 0) return fail(MXK_ERR_BAD_ARG, "plan_tokens: strides must not be negative");
     if (!offsets || (tokens > 0 && (!topk_idx || !row_of_pair || !pair_of_row)))
         return fail(MXK_ERR_BAD_ARG, "plan_tokens: pointers must be non-null");
     PlanArgs a;
@@ -261,6 +262,7 @@ int mxk_sort_tokens(const void* x, int64_t x_stride, int64_t row_bytes, const vo
                     void* rows, void* rows_sf, void* stream) {
     if (bad_tables(tokens, topk) || num_experts < 1 || num_experts > kRowsMaxExperts || row_bytes < 1 || row_bytes > kMaxRowBytes || (x_sf && (sf_bytes < 1 || sf_bytes > (1 << 24))))
         return fail(MXK_ERR_BAD_ARG, "sort_tokens: sizes out of range");
+    if (x_stride < 0 || sf_stride < 0) return fail(MXK_ERR_BAD_ARG, "sort_tokens: strides must not be negative");
     if (tokens == 0) return 0;
     if (!x || !rows || !row_of_pair || !offsets || (x_sf && !rows_sf)) return fail(MXK_ERR_BAD_ARG, "sort_tokens: pointers must be non-null");
     const int vec = common_vec(addr(x) | addr(rows) | (uint64_t)x_stride | (uint64_t)row_bytes);
@@ -291,6 +293,7 @@ int mxk_unsort_tokens(const void* rows, int32_t dtype, int64_t rows_stride, cons
                       int32_t tokens, int32_t topk, int32_t hidden, const int32_t* row_of_pair, void* y, void* stream) {
     if (bad_tables(tokens, topk) || hidden < 1 || hidden > kMaxRowBytes / 4 || dtype < MXK_DTYPE_BF16 || dtype > MXK_DTYPE_FP32)
         return fail(MXK_ERR_BAD_ARG, "unsort_tokens: sizes or type out of range");
+    if (rows_stride < 0 || weights_stride < 0) return fail(MXK_ERR_BAD_ARG, "unsort_tokens: strides must not be negative");
     if (tokens == 0) return 0;
     if (!rows || !row_of_pair || !y) return fail(MXK_ERR_BAD_ARG, "unsort_tokens: pointers must be non-null");
     UnsortArgs a;
@@ -313,6 +316,7 @@ int mxk_unsort_tokens_grad(const void* dy, int64_t dy_stride, const void* rows, 
                            void* stream) {
     if (bad_tables(tokens, topk) || num_experts < 1 || num_experts > kRowsMaxExperts || hidden < 1 || hidden > kMaxRowBytes / 4 || dtype < MXK_DTYPE_BF16 || dtype > MXK_DTYPE_FP32)
         return fail(MXK_ERR_BAD_ARG, "unsort_tokens_grad: sizes or type out of range");
+    if (dy_stride < 0 || rows_stride < 0 || weights_stride < 0) return fail(MXK_ERR_BAD_ARG, "unsort_tokens_grad: strides must not be negative");
     if (tokens == 0 || (!drows && !dweights)) return 0;
     if (!dy || !weights || !row_of_pair || !offsets || (dweights && !rows)) return fail(MXK_ERR_BAD_ARG, "unsort_tokens_grad: pointers must be non-null");
     UnsortGradArgs a;
@@ -347,6 +351,7 @@ int mxk_fp8_matmul(const MxkMatmulArgs* p, void* stream) {
     if (!p->x || !p->w || !p->out) return fail(MXK_ERR_BAD_ARG, "fp8_matmul: pointers must be non-null");
     if ((addr(p->x) | addr(p->w) | (uint64_t)p->x_stride | (uint64_t)p->w_stride) & 15 || p->x_stride < depth || p->w_stride < depth)
         return fail(MXK_ERR_BAD_ARG, "fp8_matmul: x and w need 16-byte aligned rows");
+    if (p->x_sf && rows > 1 && p->x_sf_stride < (depth + 127) / 128) return fail(MXK_ERR_BAD_ARG, "fp8_matmul: rows of x_sf overlap");
     if ((addr(p->out) & 1) || (rows > 1 && p->out_stride < cols)) return fail(MXK_ERR_BAD_ARG, "fp8_matmul: out must be bf16 rows that do not overlap");
     MmArgs a;
     std::memset(&a, 0, sizeof(a));
@@ -389,7 +394,9 @@ int mxk_fp8_matmul(const MxkMatmulArgs* p, void* stream) {
 int mxk_matmul_status(int32_t* out) {
     if (!out) return fail(MXK_ERR_BAD_ARG, "matmul_status: null argument");
     int v = 0;
-    const cudaError_t e = cudaMemcpyFromSymbol(&v, g_mm_status, sizeof(v));
+    cudaError_t e = cudaDeviceSynchronize();   // products on every stream
+    if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceSynchronize(matmul status)");
+    e = cudaMemcpyFromSymbol(&v, g_mm_status, sizeof(v));
     if (e != cudaSuccess) return cuda_fail(e, "cudaMemcpyFromSymbol(matmul status)");
     *out = v;
     return 0;

@@ -280,6 +280,7 @@ Tensor matmul(const char* fn, const Tensor& x, const MaybeTensor& x_sf, const Te
     }
     if (out_in)
         MXK_VALUE(out_in->scalar_type() == at::kBFloat16 && out_in->dim() == 2 && out_in->size(0) == rows && out_in->size(1) == cols && (cols <= 1 || out_in->stride(1) == 1) && (rows <= 1 || out_in->stride(0) >= cols), fn, ": out must be a bf16 [", rows, ", ", cols, "] tensor with contiguous rows");
+    if (out_in) MXK_VALUE(!out_in->requires_grad(), fn, ": out must not require a gradient");
     const auto at_of = [](const MaybeTensor& t) { return t ? &*t : nullptr; };
     same_device(fn, x, {&w, at_of(x_sf), at_of(w_sf), at_of(offsets), at_of(out_in)});
     const c10::cuda::CUDAGuard guard(x.device());
@@ -297,6 +298,7 @@ Tensor matmul(const char* fn, const Tensor& x, const MaybeTensor& x_sf, const Te
     a.x_format = format_code(x.scalar_type()); a.w_format = format_code(w.scalar_type());
     a.w_sf_per_row = per_row; a.zero_tail = out_in ? 0 : 1;
     done(mxk_fp8_matmul(&a, stream_of(x)), "mxk_fp8_matmul");
+    if (out_in) torch::autograd::impl::bump_version(out);   // a graph that has saved the given tensor shall notice
     return out;
 }
 

@@ -192,6 +192,46 @@ def test_special_values(rows):
     assert float(out[0, 0]) == 2.0 ** 68 and float(out[0, 5]) == 2.0 ** -32 and float(out[1, 5]) == 2.0 ** -92
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 150])
+def test_scales_on_one_operand_and_at_the_ends_of_their_range(rows):
+    g = _gen(rows + 5)
+    x, w = _data(g, (rows, 272), E4, True), _data(g, (140, 272), E4, True)
+    xs, ws = _scales(g, (rows, 3), True), _scales(g, (2, 3), True)
+    plain = x.double() @ w.double().t()
+    assert torch.equal(mm.fp8_matmul((x, xs), w), (_dequant(x, xs, False) @ w.double().t()).to(torch.bfloat16))
+    assert torch.equal(mm.fp8_matmul(x, (w, ws)), (x.double() @ _dequant(w, ws, True).t()).to(torch.bfloat16))
+    for a, b in ((0, 254), (1, 253), (254, 0), (60, 194), (254, 20), (3, 150)):   # 2^(a - 127) 2^(b - 127) is a bf16 factor
+        xs.fill_(a)
+        ws.fill_(b)
+        want = plain * 2.0 ** (a + b - 254)
+        assert torch.equal(mm.fp8_matmul((x, xs), (w, ws)), want.to(torch.bfloat16)), (a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [2, 140])
+def test_infinities_of_e5m2(rows):
+    x = torch.ones((rows, 128), device="cuda").to(E5)
+    w = torch.ones((130, 128), device="cuda").to(E5)
+    x[0, 5], x[1, 7], w[3, 9], w[4, 5] = float("inf"), float("-inf"), float("inf"), float("-inf")
+    want = x.double() @ w.double().t()
+    out = mm.fp8_matmul(x, w).double()
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out[~torch.isnan(want)], want[~torch.isnan(want)])
+
+
+@pytest.mark.gpu
+def test_given_result_is_noticed_by_autograd():
+    x = torch.ones((4, 128), device="cuda").to(E4)
+    held = torch.ones((4, 4), device="cuda", dtype=torch.bfloat16)
+    factor = torch.ones((4, 4), device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    y = (factor * held).sum()
+    mm.fp8_matmul(x, x, out=held)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with pytest.raises(ValueError, match="gradient"):
+        mm.fp8_matmul(x, x, out=factor)
+
+
 # -------------------------------------------------------------------------------- grouped
 GROUPED = [  # rows of every expert, behind: rows of nobody; cols, depth
     ([5], 0, 128, 128), ([0, 0, 3], 0, 256, 256), ([1] * 32, 0, 384, 512), ([4, 0, 1, 30, 2, 0], 5, 200, 1040),
