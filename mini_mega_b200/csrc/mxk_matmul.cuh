@@ -73,7 +73,7 @@ struct MmSmem {
     uint64_t full[kMmMaxStages], empty[kMmMaxStages];
     uint64_t sf_full[kMmMaxSfSlots], sf_empty[kMmMaxSfSlots], sf_peer[kMmMaxSfSlots];
     uint64_t acc_full[2], acc_empty[2];
-    uint64_t red_full, red_free;     // split-K exchange: all partials written / all partials read
+    uint64_t red_full, red_free;     // split-K exchange: all partials have come in / every split has added its rows up
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -82,7 +82,7 @@ struct MmSmem {
 constexpr int kMmBarriers = 2 * kMmMaxStages + 3 * kMmMaxSfSlots + 6;
 __device__ __forceinline__ uint32_t mm_barrier_count(int i, uint32_t ctas, uint32_t splits) {
     const int k = i - (2 * kMmMaxStages + 3 * kMmMaxSfSlots);
-    return k < 2 ? 1u : k < 4 ? kMmEpiWarps * ctas : kMmEpiWarps * splits;   // copies and commits; acc_empty; red_full, red_free
+    return k == 2 || k == 3 ? kMmEpiWarps * ctas : k == 5 ? kMmEpiWarps * splits : 1u;   // acc_empty; red_free; copies, commits and stores
 }
 static_assert(offsetof(MmSmem, tmem_base) == kMmBarriers * sizeof(uint64_t), "barriers first, without gaps");
 
@@ -133,8 +133,10 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void st_cluster_f32(uint32_t addr, uint32_t v) {
-    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+// A store into another CTA of the cluster that reports its four bytes to a barrier there: no fence, no
+// separate arrival (with ordinary stores, a release and an arrival the exchange of a 1 x 4096 x 6144 product took 0.6 us longer).
+__device__ __forceinline__ void st_async_b32(uint32_t addr, uint32_t v, uint32_t bar) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(v), "r"(bar) : "memory");
 }
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -495,15 +497,19 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                 uint32_t v[16];
                 tmem_ld16(tacc + c * 16, v);
                 tmem_wait_ld();
-                const uint32_t at = smem_u32(red + split * own_rows * 128 + q * 32 + lane);
+                const uint32_t at = smem_u32(red + split * own_rows * 128 + q * 32 + lane), bar = smem_u32(&S->red_full);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                     const int r = c * 16 + j;
                     if (r >= tl.valid) break;
-                    st_cluster_f32(mapa_u32(at + (uint32_t)(r >> log_splits) * 512u, (uint32_t)(r & (a.splits - 1)) * ctas + half), v[j]);
+                    const uint32_t owner = (uint32_t)(r & (a.splits - 1)) * ctas + half;
+                    st_async_b32(mapa_u32(at + (uint32_t)(r >> log_splits) * 512u, owner), v[j], mapa_u32(bar, owner));
                 }
             };
             if (a.splits > 1) {
+                // what this CTA will be sent: its rows of the tile, from every split
+                if (warp == kMmFirstEpi && lane == 0)
+                    mbar_expect_tx(&S->red_full, (uint32_t)((tl.valid + a.splits - 1 - split) >> log_splits) * (uint32_t)a.splits * 512u);
 #pragma unroll 1
                 for (int c = part; c < n_chunks; c += 2) push(c);
                 tc_fence_before();
@@ -535,7 +541,6 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                 if (lane == 0) arrive_leader(&S->acc_empty[buf]);
             }
             if (a.splits > 1) {
-                if (lane < a.splits) mbar_arrive_cluster(mapa_u32(smem_u32(&S->red_full), (uint32_t)lane * ctas + half));
                 ok = mbar_wait_cluster(&S->red_full, it & 1u, wait_ns, abort_flag);
                 ok = __all_sync(0xFFFFFFFFu, ok ? 1 : 0) != 0;
                 if (!ok) { dead = true; break; }

@@ -9,6 +9,7 @@
 // ============================================================================
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -58,6 +59,11 @@ int64_t row_bytes_apart(const Tensor& t) { return t.stride(0) * (int64_t)t.eleme
 void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 int32_t* table(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
 
+// Allocation without the dispatcher (0.3 us of 1.1), on the device of `like`.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+    return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+
 // ---- tokens sorted by expert and back ---------------------------------------------------
 int type_code(at::ScalarType t) {
     return t == at::kBFloat16 ? MXK_DTYPE_BF16 : t == at::kHalf ? MXK_DTYPE_FP16 : t == at::kFloat ? MXK_DTYPE_FP32 : -1;
@@ -74,8 +80,7 @@ std::tuple<Tensor, Tensor, Tensor> plan_tokens(const Tensor& topk_idx, int64_t n
     same_device(fn, topk_idx, {});
     const c10::cuda::CUDAGuard guard(topk_idx.device());
     const Tensor idx = rows_contiguous(topk_idx);
-    const auto opt = idx.options().dtype(at::kInt);
-    Tensor row_of_pair = at::empty({tokens, topk}, opt), pair_of_row = at::empty({tokens * topk}, opt), offsets = at::empty({num_experts + 1}, opt);
+    Tensor row_of_pair = fresh({tokens, topk}, at::kInt, idx), pair_of_row = fresh({tokens * topk}, at::kInt, idx), offsets = fresh({num_experts + 1}, at::kInt, idx);
     done(mxk_plan_tokens(idx.data_ptr(), (int32_t)idx.element_size(), idx.stride(0), (int32_t)tokens, (int32_t)topk, (int32_t)first_expert,
                          (int32_t)num_experts, table(row_of_pair), table(pair_of_row), table(offsets), stream_of(idx)),
          "mxk_plan_tokens");
@@ -109,10 +114,10 @@ Tensor sort_rows(const Tensor& x_in, const Tensor& row_of_pair, const Tensor& of
     const c10::cuda::CUDAGuard guard(x_in.device());
     const int64_t tokens = row_of_pair.size(0), topk = row_of_pair.size(1);
     const Tensor x = rows_contiguous(x_in);
-    Tensor rows = at::empty({tokens * topk, x.size(1)}, x.options()), sf;
+    Tensor rows = fresh({tokens * topk, x.size(1)}, x.scalar_type(), x), sf;
     if (sf_in.defined()) {
         sf = rows_contiguous(sf_in);
-        *rows_sf = at::empty({tokens * topk, sf.size(1)}, sf.options());
+        *rows_sf = fresh({tokens * topk, sf.size(1)}, at::kByte, sf);
     }
     done(mxk_sort_tokens(x.data_ptr(), row_bytes_apart(x), x.size(1) * (int64_t)x.element_size(), sf.defined() ? sf.data_ptr() : nullptr,
                          sf.defined() ? sf.stride(0) : 0, sf.defined() ? sf.size(1) : 0, (int32_t)tokens, (int32_t)topk,
@@ -127,7 +132,7 @@ Tensor unsort_rows(const Tensor& rows_in, const Tensor& weights_in, const Tensor
     const int64_t tokens = row_of_pair.size(0), topk = row_of_pair.size(1);
     const Tensor rows = rows_contiguous(rows_in);
     const Tensor weights = weights_in.defined() ? rows_contiguous(weights_in) : weights_in;
-    Tensor y = at::empty({tokens, rows.size(1)}, rows.options());
+    Tensor y = fresh({tokens, rows.size(1)}, rows.scalar_type(), rows);
     done(mxk_unsort_tokens(rows.data_ptr(), type_code(rows.scalar_type()), row_bytes_apart(rows),
                            weights.defined() ? static_cast<const float*>(weights.data_ptr()) : nullptr, weights.defined() ? weights.stride(0) : 0,
                            (int32_t)tokens, (int32_t)topk, (int32_t)rows.size(1), table(row_of_pair), y.data_ptr(), stream_of(rows)),
@@ -178,8 +183,8 @@ struct UnsortFunction : torch::autograd::Function<UnsortFunction> {
         const Tensor dy = rows_contiguous(grads[0]), weights = rows_contiguous(weights_in);
         const Tensor rows = saved[0].defined() ? rows_contiguous(saved[0]) : Tensor();
         Tensor drows, dweights;
-        if (ctx->saved_data["rows_grad"].toBool()) drows = at::empty({tokens * topk, dy.size(1)}, dy.options());
-        if (rows.defined()) dweights = at::empty({tokens, topk}, weights.options());
+        if (ctx->saved_data["rows_grad"].toBool()) drows = fresh({tokens * topk, dy.size(1)}, dy.scalar_type(), dy);
+        if (rows.defined()) dweights = fresh({tokens, topk}, at::kFloat, weights);
         done(mxk_unsort_tokens_grad(dy.data_ptr(), row_bytes_apart(dy), rows.defined() ? rows.data_ptr() : nullptr,
                                     rows.defined() ? row_bytes_apart(rows) : 0, type_code(dy.scalar_type()),
                                     static_cast<const float*>(weights.data_ptr()), weights.stride(0), (int32_t)tokens, (int32_t)topk,
@@ -284,7 +289,7 @@ Tensor matmul(const char* fn, const Tensor& x, const MaybeTensor& x_sf, const Te
     const auto at_of = [](const MaybeTensor& t) { return t ? &*t : nullptr; };
     same_device(fn, x, {&w, at_of(x_sf), at_of(w_sf), at_of(offsets), at_of(out_in)});
     const c10::cuda::CUDAGuard guard(x.device());
-    Tensor out = out_in ? *out_in : at::empty({rows, cols}, x.options().dtype(at::kBFloat16));
+    Tensor out = out_in ? *out_in : fresh({rows, cols}, at::kBFloat16, x);
     if (rows == 0) return out;
     MxkMatmulArgs a;
     std::memset(&a, 0, sizeof(a));
