@@ -178,6 +178,8 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
 
     // Start-up, kept short because it is a fifth of a small product: warp 0 initialises the barriers, builds the
     // group table and goes on to its first loads without waiting for the others; warp 1 meanwhile allocates TMEM.
+    // Every role waits for the kernels before this one (grid_wait) where it first touches memory and not earlier, so that
+    // its way there, instruction fetches included, lies under their end.
     grid_let_next_begin();
     if (clustered && warp != 0) cluster_arrive();
     if (warp == 0) {
@@ -195,7 +197,6 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
         }
         // Group table.  Offsets come from the device and are not trusted: clamped into [0, rows] and made
         // ascending (a running maximum), groups are disjoint whatever they held and no tile reaches outside.
-        grid_wait();   // the kernels before this one in the stream have ended: from here on memory is read
         if (!a.offsets) {
             if (lane == 0) {
                 start[0] = before[0] = 0;
@@ -203,6 +204,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                 before[1] = a.fbt.div(a.rows + a.bt_max - 1) * a.n_tiles;
             }
         } else {
+            grid_wait();   // the first read of memory
 #pragma unroll 4
             for (int e = lane; e <= a.experts; e += 32) start[e] = min(max(a.offsets[e], 0), a.rows);
             __syncwarp();
@@ -236,7 +238,6 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
             if constexpr (kPair) { tmem_alloc_pair(&S->tmem_base, kMmTmemCols); tmem_relinquish_pair(); }
             else { tmem_alloc(&S->tmem_base, kMmTmemCols); tmem_relinquish(); }
         }
-        grid_wait();
         tc_fence_before();
         asm volatile("barrier.cta.sync 1, %0;" ::"n"(kMmThreads) : "memory");
         tc_fence_after();
@@ -267,7 +268,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
         if (lane == 0) {
             uint32_t stage = 0, phase = 0;
             unsigned long long issued = 0;
-            bool dead = false;
+            bool dead = false, waited = false;
             for (int t = unit; !dead && mm_tile<kPair>(a, start, before, t, tl); t += n_units) {
                 // rows of all experts lie behind one another in the weight map; a tile that runs past its
                 // expert's last row reads the next expert's, and those output columns are not stored
@@ -290,6 +291,10 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                         if constexpr (kPair) tma_load_2d_pair(dst, map, k * 128, row, bar);
                         else tma_load_2d(dst, map, k * 128, row, &S->full[stage]);
                     };
+                    if (!waited) {
+                        grid_wait();
+                        waited = true;
+                    }
                     load(sw, tm_w, kb, w_row);
                     load(sx, tm_x, kb, x_row);
                     if (two) {
@@ -394,7 +399,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
         };
         constexpr int kXj = 4 * kXTiles;   // rows of an accumulator per lane
         uint32_t sfg = 0;
-        bool dead = false;
+        bool dead = false, waited = false;
         for (int t = unit; !dead && mm_tile<kPair>(a, start, before, t, tl); t += n_units) {
             const uint8_t* wsf = nullptr;
             int w_here = 0;   // weight rows of this CTA's half that exist
@@ -426,6 +431,10 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
             const int n_groups = g_last - g_first;
             int i0 = (int)((mine ^ sfg) & 1u);    // first group of this tile that is this warp's
             uint32_t wx[kXj], ww[4];
+            if (!waited) {
+                grid_wait();
+                waited = true;
+            }
             if (i0 < n_groups) load_group(g_first + i0, wx, ww);
             for (int i = i0; i < n_groups; i += 2) {
                 const uint32_t gg = sfg + (uint32_t)i, slot = gg % (uint32_t)a.sf_slots, par = (gg / (uint32_t)a.sf_slots) & 1u;
@@ -476,6 +485,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
         // 25.4 us like this, 27.6 with chunks turned round in shared memory and 16 bytes a lane, 32.0 with shuffles
         // and 4 bytes (rows off every alignment, 4095 columns: 28.0, 40.6, 29.0).
         const int q = warp & 3, part = (warp - kMmFirstEpi) >> 2;
+        grid_wait();   // kernels before this one may still read what is written here
         uint32_t it = 0;
         bool dead = false;
         for (int t = unit; mm_tile<kPair>(a, start, before, t, tl); t += n_units, ++it) {

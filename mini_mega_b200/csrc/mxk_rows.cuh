@@ -60,7 +60,6 @@ __host__ __device__ constexpr int plan_stride(int experts) { return experts | 1;
 
 __global__ void __launch_bounds__(kPlanThreads, 1) k_plan(const PlanArgs a) {
     grid_let_next_begin();
-    grid_wait();
     extern __shared__ int plan_smem[];
     const int stride = plan_stride(a.experts);
     int* mine = plan_smem;                        // [experts] pairs of this CTA
@@ -74,10 +73,12 @@ __global__ void __launch_bounds__(kPlanThreads, 1) k_plan(const PlanArgs a) {
     const int p1 = min(c_end, p0 + a.per_warp);
     int* my = wcnt + warp * stride;
 
+    for (int e = lane; e < a.experts; e += 32) my[e] = 0;
+    grid_wait();
+
     int keep[kPlanKeep], rank[kPlanKeep];   // ids of the slice's first pairs, and their place among the warp's pairs of that id
 #pragma unroll
     for (int i = 0; i < kPlanKeep; ++i) keep[i] = plan_id(a, p0 + i * 32 + lane, p1);
-    for (int e = lane; e < a.experts; e += 32) my[e] = 0;
     __syncwarp();
     auto count = [&](int e) -> int {
         const unsigned m = plan_peers(e, a.bits);
@@ -303,12 +304,12 @@ __device__ __forceinline__ void copy_scales(const SortArgs& a, const int* s_row,
 template <int V, int U>
 __global__ void __launch_bounds__(kRowThreads) k_sort_rows(const SortArgs a) {
     grid_let_next_begin();
-    grid_wait();
     typedef typename VecOf<V>::T T;
     __shared__ int s_row[kRowBatch];
     const RowFrame& f = a.f;
     const RowCols<V, U> c(f);
     const long long steps = (f.tokens + (long long)gridDim.x * f.tall - 1) / ((long long)gridDim.x * f.tall);
+    grid_wait();
     for (long long step0 = 0; step0 < steps; step0 += f.batch) {
         row_fetch<false>(f, nullptr, 0, step0, s_row, nullptr);
         const int here = (int)min((long long)f.batch, steps - step0);
@@ -361,7 +362,6 @@ struct UnsortArgs {
 template <int kType, int V, int U>
 __global__ void __launch_bounds__(kRowThreads, 4) k_unsort_rows(const UnsortArgs a) {
     grid_let_next_begin();
-    grid_wait();
     constexpr int kEl = elem_bytes<kType>(), kN = V / kEl;
     typedef typename VecOf<V>::T T;
     __shared__ int s_row[kRowBatch];
@@ -369,6 +369,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_unsort_rows(const UnsortArgs
     const RowFrame& f = a.f;
     const RowCols<V, U> c(f);
     const long long steps = (f.tokens + (long long)gridDim.x * f.tall - 1) / ((long long)gridDim.x * f.tall);
+    grid_wait();
     for (long long step0 = 0; step0 < steps; step0 += f.batch) {
         row_fetch<true>(f, a.w, a.w_stride, step0, s_row, s_w);
         const int here = (int)min((long long)f.batch, steps - step0);
