@@ -308,7 +308,9 @@ __device__ __forceinline__ void tma_load_2d_pair_hint(void* smem_dst, const CUte
 // ---- programmatic dependent launch ---------------------------------------------------
 // A kernel launched with the programmatic attribute may begin while its predecessor in the stream still
 // runs; everything before grid_wait() must keep to its own shared and tensor memory.  After grid_wait() the
-// predecessor has ended and its writes are visible, as behind an ordinary launch.
+// predecessor has ended and its writes are visible, as behind an ordinary launch, to ordinary loads: the read-only
+// path (__ldg) is for data that nobody writes while the kernel runs, and here the kernel already runs while its
+// predecessor writes.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

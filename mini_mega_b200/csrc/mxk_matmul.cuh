@@ -391,10 +391,10 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
         const bool x_words = a.x_sf && ((a.x_sf_stride | (long long)(reinterpret_cast<uintptr_t>(a.x_sf))) & 3) == 0;
         const bool w_words = a.w_sf && ((a.nkb | (int)(reinterpret_cast<uintptr_t>(a.w_sf) & 3)) & 3) == 0;
         auto load_word = [&](const uint8_t* p, int kb, bool words) -> uint32_t {   // p: the row's first scale byte
-            if (words && kb + 4 <= a.nkb) return __ldg(reinterpret_cast<const uint32_t*>(p + kb));
+            if (words && kb + 4 <= a.nkb) return *reinterpret_cast<const uint32_t*>(p + kb);
             uint32_t v = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v |= (kb + i < a.nkb ? (uint32_t)__ldg(p + kb + i) : 127u) << (8 * i);
+            for (int i = 0; i < 4; ++i) v |= (kb + i < a.nkb ? (uint32_t)p[kb + i] : 127u) << (8 * i);
             return v;
         };
         constexpr int kXj = 4 * kXTiles;   // rows of an accumulator per lane
