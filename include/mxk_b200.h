@@ -431,7 +431,9 @@ typedef struct MxkMatmulArgs {
     int32_t x_format, w_format;    /* MXK_FP8_*                                                    */
     int32_t w_sf_per_row;
     int32_t zero_tail;         /* grouped: clear out rows of no expert (0: they are left alone)     */
-    int32_t max_spins;         /* bound of every device wait, in units of 250 ns; 0 => 2 s         */
+    int32_t max_spins;         /* bound of every device wait in units of 250 ns, at least 8000000 (2 s); 0 => 2 s.
+                                * 4 us per 128 columns of depth come on top: a wait that expires while the
+                                * product is healthy would leave with its copies and MMAs under way    */
 } MxkMatmulArgs;
 int mxk_fp8_matmul(const MxkMatmulArgs* a, void* stream);
 /* Synchronous: 0, or the MXK_DEV_* code of the first product on this device whose wait expired (its output is

@@ -223,6 +223,11 @@ MmShape mm_shape(int64_t rows, int64_t cols, int64_t depth, int64_t experts, boo
     return best;
 }
 
+// A wait that expires ends its CTA, which must not happen while copies or MMAs of a healthy product are still on their
+// way into that CTA's memory: bounds below this are refused, and the longest wait (a tile's whole K loop) gets 4 us per
+// K block on top, more than ten times what one takes.
+constexpr int kMmLeastSpins = 8000000;
+
 int dtype_bytes(int dtype) { return dtype == MXK_DTYPE_FP32 ? 4 : 2; }
 
 }  // namespace
@@ -347,6 +352,8 @@ int mxk_fp8_matmul(const MxkMatmulArgs* p, void* stream) {
         return fail(MXK_ERR_BAD_ARG, "fp8_matmul: need depth a multiple of 16, 1 <= experts <= 1024, rows and experts * cols <= 2^30");
     if (p->x_format < MXK_FP8_E4M3 || p->x_format > MXK_FP8_E5M2 || p->w_format < MXK_FP8_E4M3 || p->w_format > MXK_FP8_E5M2)
         return fail(MXK_ERR_BAD_ARG, "fp8_matmul: operand formats are MXK_FP8_E4M3 and MXK_FP8_E5M2");
+    if (p->max_spins != 0 && p->max_spins < kMmLeastSpins)
+        return fail(MXK_ERR_BAD_ARG, "fp8_matmul: max_spins is 0 or at least 8000000 (2 s)");
     if (rows == 0) return 0;
     if (!p->x || !p->w || !p->out) return fail(MXK_ERR_BAD_ARG, "fp8_matmul: pointers must be non-null");
     if ((addr(p->x) | addr(p->w) | (uint64_t)p->x_stride | (uint64_t)p->w_stride) & 15 || p->x_stride < depth || p->w_stride < depth)
@@ -362,7 +369,7 @@ int mxk_fp8_matmul(const MxkMatmulArgs* p, void* stream) {
     a.w_sf_rows = a.w_per_row ? a.cols : (a.cols + 127) / 128;
     a.zero_tail = p->offsets && p->zero_tail;
     a.formats = ((uint32_t)p->w_format << 7) | ((uint32_t)p->x_format << 10);   // w is the MMA's A operand, x its B
-    a.wait_ns = p->max_spins > 0 ? (unsigned long long)p->max_spins * 250ull : 2000000000ull;
+    a.wait_ns = (p->max_spins ? (unsigned long long)p->max_spins * 250ull : 2000000000ull) + (unsigned long long)a.nkb * 4000ull;
 
     const MmShape sh = mm_shape(rows, cols, depth, experts, p->offsets != nullptr);
     const bool pair = sh.pair;

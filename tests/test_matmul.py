@@ -83,7 +83,7 @@ def test_c_abi_refuses_before_it_launches():
     good = dict(x=16, w=16, out=16, x_stride=128, w_stride=128, out_stride=8, rows=4, cols=8, depth=128, experts=1)
     for change in (dict(x=0), dict(w=0), dict(out=0), dict(rows=-1), dict(cols=0), dict(depth=120), dict(depth=8), dict(x_stride=112),
                    dict(w_stride=136), dict(x=24), dict(out=17), dict(out_stride=7), dict(x_format=2), dict(w_format=5),
-                   dict(offsets=16, experts=1025)):
+                   dict(offsets=16, experts=1025), dict(max_spins=1), dict(max_spins=-1), dict(max_spins=7999999)):
         assert L.mxk_fp8_matmul(ctypes.byref(_lib.MxkMatmulArgs(**{**good, **change})), None) == -1, change
         assert b"fp8_matmul" in L.mxk_last_error()
     assert L.mxk_fp8_matmul(None, None) == -1
