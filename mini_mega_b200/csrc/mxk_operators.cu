@@ -54,6 +54,7 @@ int common_vec(uint64_t bits) {
     return (int)(bits & (~bits + 1));
 }
 uint64_t addr(const void* p) { return (uint64_t)reinterpret_cast<uintptr_t>(p); }
+template <class... P> bool words(const P*... p) { return ((0 | ... | addr(p)) & 3) == 0; }   // tables and FP32 factors on 4-byte addresses
 
 // Dynamic shared memory above 48 KB has to be allowed once per kernel and device.
 int allow_smem(const void* fn, int slot, int bytes) {
@@ -242,6 +243,8 @@ int mxk_plan_tokens(const void* topk_idx, int32_t idx_bytes, int64_t idx_stride,
     if (idx_stride < 0) return fail(MXK_ERR_BAD_ARG, "plan_tokens: strides must not be negative");
     if (!offsets || (tokens > 0 && (!topk_idx || !row_of_pair || !pair_of_row)))
         return fail(MXK_ERR_BAD_ARG, "plan_tokens: pointers must be non-null");
+    if (!words(row_of_pair, pair_of_row, offsets) || addr(topk_idx) % (uint64_t)idx_bytes)
+        return fail(MXK_ERR_BAD_ARG, "plan_tokens: ids and tables must be aligned to their element type");
     PlanArgs a;
     std::memset(&a, 0, sizeof(a));
     a.idx = topk_idx; a.idx_stride = idx_stride; a.idx64 = idx_bytes == 8;
@@ -270,6 +273,7 @@ int mxk_sort_tokens(const void* x, int64_t x_stride, int64_t row_bytes, const vo
     if (x_stride < 0 || sf_stride < 0) return fail(MXK_ERR_BAD_ARG, "sort_tokens: strides must not be negative");
     if (tokens == 0) return 0;
     if (!x || !rows || !row_of_pair || !offsets || (x_sf && !rows_sf)) return fail(MXK_ERR_BAD_ARG, "sort_tokens: pointers must be non-null");
+    if (!words(row_of_pair, offsets)) return fail(MXK_ERR_BAD_ARG, "sort_tokens: tables must be aligned to their element type");
     const int vec = common_vec(addr(x) | addr(rows) | (uint64_t)x_stride | (uint64_t)row_bytes);
     SortArgs a;
     std::memset(&a, 0, sizeof(a));
@@ -307,7 +311,7 @@ int mxk_unsort_tokens(const void* rows, int32_t dtype, int64_t rows_stride, cons
     a.rows_stride = rows_stride; a.w_stride = weights_stride;
     const int row_bytes = hidden * dtype_bytes(dtype);
     const int vec = common_vec(addr(rows) | addr(y) | (uint64_t)rows_stride | (uint64_t)row_bytes);
-    if (vec < dtype_bytes(dtype)) return fail(MXK_ERR_BAD_ARG, "unsort_tokens: rows and y must be aligned to their element type");
+    if (vec < dtype_bytes(dtype) || !words(weights, row_of_pair)) return fail(MXK_ERR_BAD_ARG, "unsort_tokens: tensors must be aligned to their element type");
     const dim3 grid = row_frame(a.f, tokens, topk, row_bytes, vec, unroll_of(vec), row_of_pair);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == MXK_DTYPE_BF16) return unsort_launch<kTypeBf16>(a, vec, grid, st);
@@ -334,7 +338,7 @@ int mxk_unsort_tokens_grad(const void* dy, int64_t dy_stride, const void* rows, 
     if (drows) bits |= addr(drows);
     if (dweights) bits |= addr(rows) | (uint64_t)rows_stride;
     const int vec = common_vec(bits);
-    if (vec < dtype_bytes(dtype)) return fail(MXK_ERR_BAD_ARG, "unsort_tokens_grad: tensors must be aligned to their element type");
+    if (vec < dtype_bytes(dtype) || !words(weights, row_of_pair, offsets, dweights)) return fail(MXK_ERR_BAD_ARG, "unsort_tokens_grad: tensors must be aligned to their element type");
     a.vecs = a.row_bytes / vec;
     a.team = 1;   // warps per token: as many as the row has columns for
     while (a.team < 8 && a.vecs > 32 * a.team) a.team *= 2;
@@ -358,6 +362,7 @@ int mxk_fp8_matmul(const MxkMatmulArgs* p, void* stream) {
     if (!p->x || !p->w || !p->out) return fail(MXK_ERR_BAD_ARG, "fp8_matmul: pointers must be non-null");
     if ((addr(p->x) | addr(p->w) | (uint64_t)p->x_stride | (uint64_t)p->w_stride) & 15 || p->x_stride < depth || p->w_stride < depth)
         return fail(MXK_ERR_BAD_ARG, "fp8_matmul: x and w need 16-byte aligned rows");
+    if (!words(p->offsets)) return fail(MXK_ERR_BAD_ARG, "fp8_matmul: offsets must be aligned to their element type");
     if (p->x_sf && rows > 1 && p->x_sf_stride < (depth + 127) / 128) return fail(MXK_ERR_BAD_ARG, "fp8_matmul: rows of x_sf overlap");
     if ((addr(p->out) & 1) || (rows > 1 && p->out_stride < cols)) return fail(MXK_ERR_BAD_ARG, "fp8_matmul: out must be bf16 rows that do not overlap");
     MmArgs a;

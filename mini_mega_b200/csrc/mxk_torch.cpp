@@ -259,6 +259,7 @@ Tensor matmul(const char* fn, const Tensor& x, const MaybeTensor& x_sf, const Te
     const int64_t w_dim = offsets ? 3 : 2;
     MXK_TYPE(format_code(x.scalar_type()) >= 0, fn, ": x must be a float8_e4m3fn, float8_e5m2 (or raw uint8 E4M3) tensor");
     MXK_TYPE(format_code(w.scalar_type()) >= 0, fn, ": w must be a float8_e4m3fn, float8_e5m2 (or raw uint8 E4M3) tensor");
+    MXK_TYPE(!at::GradMode::is_enabled() || !(x.requires_grad() || w.requires_grad()), fn, ": has no gradient: detach the operands, or call it under no_grad");
     MXK_VALUE(x.dim() == 2, fn, ": x must have 2 dimensions, got ", x.sizes());
     MXK_VALUE(w.dim() == w_dim, fn, ": w must have ", w_dim, " dimensions, got ", w.sizes());
     MXK_TYPE(!x_sf || x_sf->scalar_type() == at::kByte, fn, ": x scales must be uint8 exponents");

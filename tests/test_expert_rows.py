@@ -56,6 +56,11 @@ def _cpu_plan(tokens=4, topk=2, experts=3):
     return mm.ExpertPlan(*plain_plan(np.zeros((tokens, topk), np.int64), experts))
 
 
+@pytest.fixture(scope="module")
+def built():
+    _lib.build()
+
+
 @pytest.mark.parametrize("make, err", [
     (lambda: mm.plan_tokens_by_expert(torch.zeros(4, 2), 3), TypeError),
     (lambda: mm.plan_tokens_by_expert(torch.zeros(4, dtype=torch.int64), 3), ValueError),
@@ -82,7 +87,7 @@ def _cpu_plan(tokens=4, topk=2, experts=3):
     (lambda: mm.unsort_tokens_by_expert(torch.zeros(8, 8), _cpu_plan(), torch.zeros(2, 4)), ValueError),
     (lambda: mm.unsort_tokens_by_expert(torch.zeros(8, 8), _cpu_plan(), torch.zeros(4, 2)), ValueError),
 ])
-def test_refusals(make, err):
+def test_refusals(built, make, err):
     with pytest.raises(err):
         make()
 
@@ -99,6 +104,19 @@ def test_c_abi_refuses_before_it_launches():
     assert L.mxk_unsort_tokens(one, 3, 16, None, 0, 4, 2, 8, one, one, None) == -1
     assert L.mxk_unsort_tokens(17, 0, 16, None, 0, 4, 2, 8, one, one, None) == -1
     assert L.mxk_unsort_tokens_grad(one, 16, None, 16, 0, one, 2, 4, 2, 8, 8, one, one, one, one, None) == -1
+    # addresses off their element's alignment, which would fault
+    assert L.mxk_plan_tokens(20, 8, 2, 4, 2, 0, 8, one, one, one, None) == -1
+    assert L.mxk_plan_tokens(18, 4, 2, 4, 2, 0, 8, one, one, one, None) == -1
+    for tables in ((18, 16, 16), (16, 18, 16), (16, 16, 18)):
+        assert L.mxk_plan_tokens(one, 8, 2, 4, 2, 0, 8, *tables, None) == -1
+    assert L.mxk_sort_tokens(one, 16, 16, None, 0, 0, 4, 2, 8, 18, one, one, None, None) == -1
+    assert L.mxk_sort_tokens(one, 16, 16, None, 0, 0, 4, 2, 8, one, 18, one, None, None) == -1
+    assert L.mxk_unsort_tokens(one, 0, 16, 18, 2, 4, 2, 8, one, one, None) == -1
+    assert L.mxk_unsort_tokens(one, 0, 16, one, 2, 4, 2, 8, 18, one, None) == -1
+    for k in (5, 11, 12, 14):
+        args = [one, 16, one, 16, 0, one, 2, 4, 2, 8, 8, one, one, one, one, None]
+        args[k] = 18
+        assert L.mxk_unsort_tokens_grad(*args) == -1, k
     assert len(L.mxk_last_error()) > 0
 
 

@@ -29,6 +29,11 @@ def _sf(*shape):
 _OFF = torch.zeros(4, dtype=torch.int32)
 
 
+@pytest.fixture(scope="module")
+def built():
+    _lib.build()
+
+
 @pytest.mark.parametrize("make, err", [
     (lambda: mm.fp8_matmul(torch.zeros(4, 256), _x()), TypeError),
     (lambda: mm.fp8_matmul(_x(), torch.zeros(4, 256, dtype=torch.bfloat16)), TypeError),
@@ -50,6 +55,9 @@ _OFF = torch.zeros(4, dtype=torch.int32)
     (lambda: mm.fp8_matmul(_x(), _x(), out=torch.zeros((4, 5), dtype=torch.bfloat16)), ValueError),
     (lambda: mm.fp8_matmul(_x(), _x(), out=torch.zeros((4, 8), dtype=torch.bfloat16)[:, ::2]), ValueError),
     (lambda: mm.fp8_matmul(_x(), _x()), ValueError),                       # CPU tensors
+    (lambda: mm.fp8_matmul(_x().float().requires_grad_().to(E4), _x()), TypeError),      # no gradient would come back
+    (lambda: mm.fp8_matmul(_x(), _x().requires_grad_()), TypeError),
+    (lambda: mm.fp8_grouped_matmul(_x().requires_grad_(), torch.zeros((3, 8, 256), dtype=E4), _OFF), TypeError),
     (lambda: mm.fp8_grouped_matmul(_x(), _x(), _OFF), ValueError),         # w without an expert dimension
     (lambda: mm.fp8_grouped_matmul(_x(), torch.zeros((3, 8, 256), dtype=E4), None), TypeError),
     (lambda: mm.fp8_grouped_matmul(_x(), torch.zeros((4, 8, 256), dtype=E4), _OFF), ValueError),
@@ -58,7 +66,7 @@ _OFF = torch.zeros(4, dtype=torch.int32)
     (lambda: mm.fp8_grouped_matmul(_x(), (torch.zeros((3, 8, 256), dtype=E4), _sf(1, 2)), _OFF), ValueError),
     (lambda: mm.fp8_grouped_matmul(_x(), torch.zeros((3, 8, 256), dtype=E4), _OFF), ValueError),
 ])
-def test_refusals(make, err):
+def test_refusals(built, make, err):
     with pytest.raises(err):
         make()
 
@@ -83,7 +91,8 @@ def test_c_abi_refuses_before_it_launches():
     good = dict(x=16, w=16, out=16, x_stride=128, w_stride=128, out_stride=8, rows=4, cols=8, depth=128, experts=1)
     for change in (dict(x=0), dict(w=0), dict(out=0), dict(rows=-1), dict(cols=0), dict(depth=120), dict(depth=8), dict(x_stride=112),
                    dict(w_stride=136), dict(x=24), dict(out=17), dict(out_stride=7), dict(x_format=2), dict(w_format=5),
-                   dict(offsets=16, experts=1025), dict(max_spins=1), dict(max_spins=-1), dict(max_spins=7999999)):
+                   dict(offsets=16, experts=1025), dict(max_spins=1), dict(max_spins=-1), dict(max_spins=7999999),
+                   dict(offsets=18)):
         assert L.mxk_fp8_matmul(ctypes.byref(_lib.MxkMatmulArgs(**{**good, **change})), None) == -1, change
         assert b"fp8_matmul" in L.mxk_last_error()
     assert L.mxk_fp8_matmul(None, None) == -1
