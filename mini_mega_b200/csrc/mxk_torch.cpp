@@ -64,6 +64,14 @@ Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
     return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
 }
 
+// Part of an int32 tensor's memory as a tensor of its own: 0.1 us where an allocation takes 0.8.
+Tensor part_of(const Tensor& whole, int64_t first, at::IntArrayRef sizes) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(first);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    return t;
+}
+
 // ---- tokens sorted by expert and back ---------------------------------------------------
 int type_code(at::ScalarType t) {
     return t == at::kBFloat16 ? MXK_DTYPE_BF16 : t == at::kHalf ? MXK_DTYPE_FP16 : t == at::kFloat ? MXK_DTYPE_FP32 : -1;
@@ -80,7 +88,9 @@ std::tuple<Tensor, Tensor, Tensor> plan_tokens(const Tensor& topk_idx, int64_t n
     same_device(fn, topk_idx, {});
     const c10::cuda::CUDAGuard guard(topk_idx.device());
     const Tensor idx = rows_contiguous(topk_idx);
-    Tensor row_of_pair = fresh({tokens, topk}, at::kInt, idx), pair_of_row = fresh({tokens * topk}, at::kInt, idx), offsets = fresh({num_experts + 1}, at::kInt, idx);
+    const int64_t pairs = tokens * topk;
+    const Tensor tables = fresh({2 * pairs + num_experts + 1}, at::kInt, idx);
+    Tensor row_of_pair = part_of(tables, 0, {tokens, topk}), pair_of_row = part_of(tables, pairs, {pairs}), offsets = part_of(tables, 2 * pairs, {num_experts + 1});
     done(mxk_plan_tokens(idx.data_ptr(), (int32_t)idx.element_size(), idx.stride(0), (int32_t)tokens, (int32_t)topk, (int32_t)first_expert,
                          (int32_t)num_experts, table(row_of_pair), table(pair_of_row), table(offsets), stream_of(idx)),
          "mxk_plan_tokens");
