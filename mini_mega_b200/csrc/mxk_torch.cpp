@@ -54,7 +54,10 @@ void same_device(const char* fn, const Tensor& first, std::initializer_list<cons
     MXK_VALUE(d.is_cuda(), fn, " runs on CUDA tensors only, got ", d.str());
 }
 
-Tensor rows_contiguous(const Tensor& t) { return t.stride(1) == 1 || t.size(1) == 1 ? t : t.contiguous(); }
+Tensor rows_contiguous(const Tensor& t) {
+    if (t.is_neg()) return t.resolve_neg().contiguous();   // a view that carries its sign in a flag
+    return t.stride(1) == 1 || t.size(1) == 1 ? t : t.contiguous();
+}
 int64_t row_bytes_apart(const Tensor& t) { return t.stride(0) * (int64_t)t.element_size(); }
 void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 int32_t* table(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
@@ -296,7 +299,7 @@ Tensor matmul(const char* fn, const Tensor& x, const MaybeTensor& x_sf, const Te
     }
     if (out_in)
         MXK_VALUE(out_in->scalar_type() == at::kBFloat16 && out_in->dim() == 2 && out_in->size(0) == rows && out_in->size(1) == cols && (cols <= 1 || out_in->stride(1) == 1) && (rows <= 1 || out_in->stride(0) >= cols), fn, ": out must be a bf16 [", rows, ", ", cols, "] tensor with contiguous rows");
-    if (out_in) MXK_VALUE(!out_in->requires_grad(), fn, ": out must not require a gradient");
+    if (out_in) MXK_VALUE(!out_in->requires_grad() && (!out_in->is_inference() || c10::InferenceMode::is_enabled()), fn, ": out must not require a gradient, nor be an inference tensor outside inference mode");
     const auto at_of = [](const MaybeTensor& t) { return t ? &*t : nullptr; };
     same_device(fn, x, {&w, at_of(x_sf), at_of(w_sf), at_of(offsets), at_of(out_in)});
     const c10::cuda::CUDAGuard guard(x.device());

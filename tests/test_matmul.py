@@ -29,6 +29,11 @@ def _sf(*shape):
 _OFF = torch.zeros(4, dtype=torch.int32)
 
 
+def _inference_out():
+    with torch.inference_mode():
+        return torch.zeros((4, 4), dtype=torch.bfloat16)
+
+
 @pytest.fixture(scope="module")
 def built():
     _lib.build()
@@ -54,6 +59,7 @@ def built():
     (lambda: mm.fp8_matmul(_x(), _x(), out=torch.zeros(4, 4)), ValueError),
     (lambda: mm.fp8_matmul(_x(), _x(), out=torch.zeros((4, 5), dtype=torch.bfloat16)), ValueError),
     (lambda: mm.fp8_matmul(_x(), _x(), out=torch.zeros((4, 8), dtype=torch.bfloat16)[:, ::2]), ValueError),
+    (lambda: mm.fp8_matmul(_x(), _x(), out=_inference_out()), ValueError),
     (lambda: mm.fp8_matmul(_x(), _x()), ValueError),                       # CPU tensors
     (lambda: mm.fp8_matmul(_x().float().requires_grad_().to(E4), _x()), TypeError),      # no gradient would come back
     (lambda: mm.fp8_matmul(_x(), _x().requires_grad_()), TypeError),

@@ -81,6 +81,30 @@ def test_capture_of_the_whole_run_follows_its_inputs():
         assert torch.equal(held, _apart(x, x_sf, idx, weights, l1, l2, 8))
 
 
+def test_inference_mode_and_sign_flag_views():
+    """Tables, rows and results made in inference mode; inputs that are views with their sign in a flag."""
+    case = orc.gen_case(1, 8, 2, 512, 256, 33, seed=5, routing="logits", scaled=True)
+    x, x_sf = _dev(case.x[0][:33], torch.float8_e4m3fn), _dev(case.x_sf[0][:33])
+    idx, weights = _dev(case.topk_idx[0][:33]), _dev(case.topk_w[0][:33])
+    l1, l2 = (_dev(case.w1).view(torch.float8_e4m3fn), _dev(case.w1_sf)), (_dev(case.w2).view(torch.float8_e4m3fn), _dev(case.w2_sf))
+    want = _apart(x, x_sf, idx, weights, l1, l2, 8)
+    with torch.inference_mode():
+        plan = mm.plan_tokens_by_expert(idx, 8)
+        got = _apart(x, x_sf, idx, weights, l1, l2, 8)
+        out = torch.zeros((33, 512), dtype=torch.bfloat16, device="cuda")
+        assert mm.fp8_matmul(x, l1[0][0], out=out) is not None
+        assert plan.offsets.is_inference() and out.is_inference()
+        assert torch.equal(out, mm.fp8_matmul(x, l1[0][0]))
+        assert torch.equal(got, want)
+    flagged = torch.view_as_complex(torch.arange(33 * 20 * 2, device="cuda").float().view(33, 20, 2)).conj().imag
+    assert flagged.is_neg()
+    plan = mm.plan_tokens_by_expert(idx, 8)
+    rows = mm.sort_tokens_by_expert(flagged, plan)
+    assert torch.equal(rows, mm.sort_tokens_by_expert(flagged.resolve_neg().contiguous(), plan))
+    sign = torch.view_as_complex(torch.ones((33, 2, 2), device="cuda")).conj().imag
+    assert torch.equal(mm.unsort_tokens_by_expert(rows, plan, sign), -mm.unsort_tokens_by_expert(rows, plan))
+
+
 def test_training_step():
     tokens, topk, experts, hidden, inter = 50, 3, 5, 24, 32
     g = torch.Generator().manual_seed(8)
