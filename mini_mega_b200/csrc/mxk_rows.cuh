@@ -22,8 +22,9 @@ constexpr int kRowsMaxExperts = 1024;
 // 2 hands the rows out.  Bound by the latency of its steps, not by bytes, so each step is one round trip: ids and
 // places of a slice of up to 128 pairs stay in registers, counters are read in batches, the peers' counts are requested
 // together.  Up to 1024 pairs one CTA of few warps, up to 16384 a cluster of 8 CTAs, beyond that of 16 (1024 pairs, 256
-// experts: 1 CTA 6.3 us, 8 CTAs 8.3; 32768 pairs, 32 experts: 8 CTAs 10.3 us, 16 CTAs 8.3; 524288 pairs, 128
-// experts: 115 and 62 us, with match.any in place of the ballots 147 and 80).
+// experts: 1 CTA 6.3 us, 8 CTAs 8.3; 32768 pairs, 32 experts: 8 CTAs 10.3 us, 16 CTAs 8.3; of which a launch that
+// starts under its predecessor's end hides some 2 us).  Long slices: pass 1 only needs numbers, so beyond the kept ids it adds them
+// with shared-memory atomics (524288 pairs, 128 experts: 45 us, with ballots there too 60, with match.any 80).
 struct PlanArgs {
     const void* idx;
     long long idx_stride;      // elements between two tokens' ids
@@ -97,7 +98,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) k_plan(const PlanArgs a) {
         for (int i = 0; i < kPlanKeep; ++i) e[i] = plan_id(a, p + i * 32 + lane, p1);
 #pragma unroll
         for (int i = 0; i < kPlanKeep; ++i)
-            if (p + i * 32 < p1) (void)count(e[i]);
+            if (e[i] >= 0) atomicAdd(my + e[i], 1);   // a number, whatever the order
     }
     __syncthreads();
     const int e = threadIdx.x;   // one expert per thread from here on
@@ -171,7 +172,9 @@ __global__ void __launch_bounds__(kPlanThreads, 1) k_plan(const PlanArgs a) {
     if (p0 + kPlanKeep * 32 < p1) {   // the rest is ranked again: first past the kept ones, then on
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < kPlanKeep; ++i) (void)count(keep[i]);
+        for (int i = 0; i < kPlanKeep; ++i)
+            if (keep[i] >= 0) atomicAdd(my + keep[i], 1);
+        __syncwarp();
 #pragma unroll 1
         for (int p = p0 + kPlanKeep * 32; p < p1; p += kPlanKeep * 32) {
             int id[kPlanKeep];
