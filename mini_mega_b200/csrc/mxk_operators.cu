@@ -179,18 +179,21 @@ int unsort_grad_launch(const UnsortGradArgs& a, int vec, int grid, cudaStream_t 
 int unroll_of(int vec) { return vec >= 16 ? 1 : vec == 8 ? 2 : 4; }
 
 // How a product is cut: CTA pairs or single CTAs, rows of x per tile, CTAs that share a tile's K extent.  The cut
-// with the least estimated time, from the parts that were measured on a B200 (us; K blocks of 128):
-//   start, tile hand-over and end     single 5.6 and 0.006 per row of x in a tile, pair 8.0
+// with the least estimated time, from the parts that were measured on a B200 (us, launches back to back; K blocks of 128;
+// `full`: the part of the GPU that has a tile):
+//   start and end                     single 3.5 + full (0.6 + 0.014 x rows of x in a tile), pair 5.0 + 0.022 x rows x full
 //   one K block of a tile             single 153 ns + 0.64 ns x rows (32 rows: 173, 64: 195, 128: 234), pair 145 ns +
 //                                     0.6 ns x rows (128 rows: 230, 192: 267, 224: 279)
-//   partial sums between splits       1.0 + 0.25 x splits + 0.012 x rows
+//   a further round of tiles          0.25
+//   partial sums between splits       0.8 + full (1.1 + 0.018 x rows)
 // and, beside them, the operands' way from memory (6.3 TB/s) and, for every tile of rows after a group's first, its
-// weights' way from L2 once more (12 TB/s).  Both sides, measured: 1 x 4096 x 6144 in 1 / 2 / 4 splits 12.8 / 10.6 /
-// 9.6 us; 128 x 2048 x 6144 tiles of 128 rows in 4 splits 12.5, of 64 rows 11.5; 512 x 4096 x 7168 single 19.4, pairs
-// 22.3; 2048 x 4096 x 7168 single 58.7, pairs 53.8; 32 groups of 200 rows x 4096 x 7168 pairs with one tile a group
-// 195, with two 272, single CTAs with two 254.  Splits only while every tile runs at once: a second round costs 7 us
-// (20 groups of 40 rows x 1000 x 2992: 21 us without splits, 24 in two, 45 in four), and 8 of them only for a few
-// tiles, because few clusters of eight fit the GPU at once (1 x 2048 x 6144: 14.3 us, in four 8.8).
+// weights' way from L2 once more (12 TB/s).  Both sides, measured: 1 x 4096 x 6144 in 1 / 2 / 4 splits 11.3 / 8.7 /
+// 8.0 us; 16 x 1024 x 2048 6.3 / 6.5 / 5.5; 128 x 4096 x 7168 tiles of 64 rows in 2 splits 12.2, of 32 rows unsplit 13.6;
+// 512 x 4096 x 7168 single 17.5, pairs 20.1; 2048 x 4096 x 7168 single 57, pairs 52; 32 groups of 200 rows x 4096 x 7168
+// pairs with one tile a group 192, with two 282, single CTAs with two 252.  Splits only while every tile runs at once: a
+// second round costs 7 us (20 groups of 40 rows x 1000 x 2992: 21 us without splits, 24 in two, 45 in four), and 8 of them
+// only for a few tiles, because few clusters of eight fit the GPU at once (1 x 2048 x 6144: 14.3 us, in four 8.8).
+// Of 55 products, dense and grouped, 53 ran within 5 % of the best of all cuts, the others within 11 %.
 struct MmShape { bool pair; int bt, splits; };
 MmShape mm_shape(int64_t rows, int64_t cols, int64_t depth, int64_t experts, bool grouped) {
     const int nkb = (int)((depth + 127) / 128), k_groups = (nkb + 3) / 4;
@@ -207,9 +210,10 @@ MmShape mm_shape(int64_t rows, int64_t cols, int64_t depth, int64_t experts, boo
         if (splits > 1 && (grouped ? tiles + tiles / 2 : tiles) > units) return;
         const double block = pair ? 0.145 + 0.0006 * real : 0.153 + 0.00064 * bt;
         const double compute = (double)waves * (double)((nkb + splits - 1) / splits) * block;
-        const double time = (pair ? 8.0 : 5.6 + 0.006 * real) + std::max(compute, grouped ? memory : 0.0) +
-                            (grouped ? (double)(tt - 1) * weights / 12e6 : 0.0) +
-                            (splits > 1 ? 1.0 + 0.25 * splits + 0.012 * real : 0.0);
+        const double full = std::min(1.0, (double)tiles * splits / (double)(pair ? kSms / 2 : kSms));   // of the GPU that works at once
+        const double time = (pair ? 5.0 + 0.022 * real * full : 3.5 + (0.6 + 0.014 * real) * full) +
+                            std::max(compute, grouped ? memory : 0.0) + (grouped ? (double)(tt - 1) * weights / 12e6 : 0.0) +
+                            0.25 * (double)(waves - 1) + (splits > 1 ? 0.8 + (1.1 + 0.018 * real) * full : 0.0);
         if (time < least) { least = time; best = MmShape{pair, bt, splits}; }
     };
     for (int bt : {16, 32, 48, 64, 96, 128}) {
