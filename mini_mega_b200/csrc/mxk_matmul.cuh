@@ -87,35 +87,48 @@ __device__ __forceinline__ uint32_t mm_barrier_count(int i, uint32_t ctas, uint3
 static_assert(offsetof(MmSmem, tmem_base) == kMmBarriers * sizeof(uint64_t), "barriers first, without gaps");
 
 struct MmTile {
-    int group, w_row, x_row, bt, valid;    // w_row: first weight row inside the group; x_row, bt: rows of x
+    int group = 0, w_row, x_row, bt, valid;    // w_row: first weight row inside the group; x_row, bt: rows of x
+    int n = -1, row0, tile0, tt, per;          // of the group: rows, first row, first tile, tiles over the rows, rows of a tile
 };
 
 // status word of the products on this device: 0, or the first wait that expired
 __device__ int g_mm_status = 0;
 
-// Tile t of the list: groups in order; inside a group the operand with fewer rows turns fastest,
-// so that the other one is read from memory once while the first stays in L2.
+// Tile t of the list, found by a whole warp from the tile before it (t only grows): groups in order; inside a group the
+// operand with fewer rows turns fastest, so that the other one is read from memory once while the first stays in L2.  Every
+// role does this between two tiles, so it is kept short: one round trip to shared memory per 32 groups that are passed, and what
+// belongs to the group is computed once (a binary search and two divisions per tile: 800 clocks under load).
 template <bool kPair>
-__device__ __forceinline__ bool mm_tile(const MmArgs& a, const int* start, const int* before, int t, MmTile& o) {
+__device__ __forceinline__ bool mm_tile(const MmArgs& a, const int* start, const int* before, int t, int lane, MmTile& o) {
     if (t >= before[a.experts]) return false;
-    int lo = 0, hi = a.experts;   // last group with before[g] <= t; empty groups share a value with their successor
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (before[mid] <= t) lo = mid; else hi = mid;
+    int lo = o.group;   // the last group with before[g] <= t; empty groups share a value with their successor
+    for (;;) {
+        const int e = lo + 1 + lane;
+        const unsigned passed = __ballot_sync(0xFFFFFFFFu, e < a.experts && before[e] <= t);
+        lo += __popc(passed);
+        if (passed != 0xFFFFFFFFu) break;
     }
-    const int n = start[lo + 1] - start[lo], i = t - before[lo];
-    int xt = 0, wt = i, per = n;
-    if (n > a.bt_max) {
-        const int tt = a.fbt.div(n + a.bt_max - 1);
-        if (n <= a.cols) { wt = i / tt; xt = i - wt * tt; }
+    if (lo != o.group || o.n < 0) {
+        o.group = lo;
+        o.row0 = start[lo];
+        o.tile0 = before[lo];
+        o.n = o.per = start[lo + 1] - o.row0;
+        o.tt = 1;
+        if (o.n > a.bt_max) {
+            o.tt = a.fbt.div(o.n + a.bt_max - 1);
+            o.per = (o.n + o.tt - 1) / o.tt;
+        }
+        o.bt = (o.per + 15) & ~15;   // the group's rows spread evenly over its tiles
+    }
+    int xt = 0, wt = t - o.tile0;
+    if (o.tt > 1) {
+        const int i = wt;
+        if (o.n <= a.cols) { wt = i / o.tt; xt = i - wt * o.tt; }
         else { xt = a.fnt.div(i); wt = i - xt * a.n_tiles; }
-        per = (n + tt - 1) / tt;
     }
-    o.group = lo;
-    o.bt = (per + 15) & ~15;   // the group's rows spread evenly over its tiles
     o.w_row = wt * (kPair ? 256 : 128);
-    o.x_row = start[lo] + xt * o.bt;
-    o.valid = min(o.bt, n - xt * o.bt);
+    o.x_row = o.row0 + xt * o.bt;
+    o.valid = min(o.bt, o.n - xt * o.bt);
     return true;
 }
 
@@ -137,6 +150,15 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
 // separate arrival (with ordinary stores, a release and an arrival the exchange of a 1 x 4096 x 6144 product took 0.6 us longer).
 __device__ __forceinline__ void st_async_b32(uint32_t addr, uint32_t v, uint32_t bar) {
     asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(v), "r"(bar) : "memory");
+}
+// v = the word at p if `has`, else v as it was
+__device__ __forceinline__ void ld_if(uint32_t& v, const void* p, bool has) {
+    asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %2, 0;\n@q ld.global.b32 %0, [%1];\n}\n" : "+r"(v) : "l"(p), "r"((int)has));
+}
+// An arrival, here or in another CTA of the cluster, that orders no memory: what it reports are reads of tensor memory,
+// which tcgen05.wait and tcgen05.fence have ordered before it.
+__device__ __forceinline__ void mbar_arrive_relaxed(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -260,16 +282,20 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
         if constexpr (kPair) mbar_arrive_cluster(mapa_u32(smem_u32(bar), first));
         else mbar_arrive(bar);
     };
+    auto drained = [&](uint64_t* bar) {
+        if constexpr (kPair) mbar_arrive_relaxed(mapa_u32(smem_u32(bar), first));
+        else mbar_arrive(bar);
+    };
     MmTile tl;
     bool left = false;   // this thread has arrived at the closing cluster barrier
 
     if (warp == 0) {
         // --------------------------------------------------------------- TMA producer
-        if (lane == 0) {
-            uint32_t stage = 0, phase = 0;
-            unsigned long long issued = 0;
-            bool dead = false, waited = false;
-            for (int t = unit; !dead && mm_tile<kPair>(a, start, before, t, tl); t += n_units) {
+        uint32_t stage = 0, phase = 0;
+        unsigned long long issued = 0;
+        bool dead = false, waited = false;
+        for (int t = unit; mm_tile<kPair>(a, start, before, t, lane, tl); t += n_units) {
+            if (lane == 0) {
                 // rows of all experts lie behind one another in the weight map; a tile that runs past its
                 // expert's last row reads the next expert's, and those output columns are not stored
                 const int w_row = (int)((long long)tl.group * a.cols) + tl.w_row + 128 * (int)half;
@@ -305,6 +331,9 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                     if (++stage == (uint32_t)a.n_stages) { stage = 0; phase ^= 1; }
                 }
             }
+            if (__any_sync(0xFFFFFFFFu, dead ? 1 : 0)) break;
+        }
+        if (lane == 0) {
             if (dead || *abort_flag) {
                 if (dead) mm_raise(S, MXK_DEV_TIMEOUT_PIPE);
                 // nothing may still be on its way into this shared memory when the CTA ends
@@ -339,7 +368,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                 if constexpr (kPair) umma_commit_pair_at(smem_u32(bar), first);
                 else umma_commit(bar);
             };
-            for (int t = unit; !dead && mm_tile<kPair>(a, start, before, t, tl); t += n_units, ++it) {
+            for (int t = unit; !dead && mm_tile<kPair>(a, start, before, t, lane, tl); t += n_units, ++it) {
                 const uint32_t idesc0 = umma_idesc_mx_e4m3(kPair ? 256 : 128, tl.bt, 0, 0) | a.formats;
                 const uint32_t buf = it & 1u, use = it >> 1;
                 const uint32_t tacc = tmem_base + buf * (uint32_t)a.bt_max;
@@ -390,91 +419,102 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
         const uint32_t mine = (uint32_t)(warp - 2);
         const bool x_words = a.x_sf && ((a.x_sf_stride | (long long)(reinterpret_cast<uintptr_t>(a.x_sf))) & 3) == 0;
         const bool w_words = a.w_sf && ((a.nkb | (int)(reinterpret_cast<uintptr_t>(a.w_sf) & 3)) & 3) == 0;
-        auto load_word = [&](const uint8_t* p, int kb, bool words) -> uint32_t {   // p: the row's first scale byte
-            if (words && kb + 4 <= a.nkb) return *reinterpret_cast<const uint32_t*>(p + kb);
-            uint32_t v = 0;
+        // Four scale bytes of a row from K block kb on; 127 where there is no row (`has`) or no further block.  The word
+        // form leaves the load under way: a value chosen after the load would wait for it here.
+        auto load_word = [&](uint32_t& v, const uint8_t* p, bool has, int kb, bool words) {
+            v = 0x7F7F7F7Fu;
+            if (words && kb + 4 <= a.nkb) {
+                ld_if(v, p + kb, has);
+            } else if (has) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v |= (kb + i < a.nkb ? (uint32_t)p[kb + i] : 127u) << (8 * i);
-            return v;
+                for (int i = 0; i < 4; ++i)
+                    if (kb + i < a.nkb) v = (v & ~(0xFFu << (8 * i))) | ((uint32_t)p[kb + i] << (8 * i));
+            }
         };
         constexpr int kXj = 4 * kXTiles;   // rows of an accumulator per lane
-        uint32_t sfg = 0;
-        bool dead = false, waited = false;
-        for (int t = unit; !dead && mm_tile<kPair>(a, start, before, t, tl); t += n_units) {
-            const uint8_t* wsf = nullptr;
-            int w_here = 0;   // weight rows of this CTA's half that exist
-            if (a.w_sf) {
-                const int r0 = tl.w_row + 128 * (int)half;
-                w_here = a.cols - r0;
-                const long long plane = (long long)tl.group * a.w_sf_rows;
-                wsf = a.w_sf + (plane + (a.w_per_row ? r0 : r0 >> 7)) * a.nkb;
+        // The loads run one group ahead of the copies, over the end of a tile too: group n of this CTA's list is group
+        // n % n_groups of its tile n / n_groups.
+        const int n_groups = g_last - g_first;
+        const uint8_t *wsf = nullptr, *xsf = nullptr;
+        int t = unit - n_units, w_here = 0, valid = 0, g = n_groups + (int)mine;   // w_here: weight rows of this CTA's half that exist
+        uint32_t wx[kXj], ww[4];
+        bool waited = false;
+        auto load_next = [&]() -> bool {   // this warp's next group, if there is one
+            bool entered = false;
+            while (g >= n_groups) {
+                g -= n_groups;
+                t += n_units;
+                entered = true;
             }
-            const uint8_t* xsf = a.x_sf ? a.x_sf + (long long)tl.x_row * a.x_sf_stride : nullptr;
-            auto load_group = [&](int g, uint32_t (&wx)[kXj], uint32_t (&ww)[4]) {
-                const int kb = g * 4;
-#pragma unroll
-                for (int j = 0; j < kXj; ++j) {
-                    const int r = lane + 32 * j;
-                    wx[j] = (xsf && r < tl.valid) ? load_word(xsf + (long long)r * a.x_sf_stride, kb, x_words) : 0x7F7F7F7Fu;
-                }
-                if (!a.w_per_row) {   // a 128 x 128 block: one word for all rows
-                    const uint32_t v = (wsf && w_here > 0) ? load_word(wsf, kb, w_words) : 0x7F7F7F7Fu;
-                    ww[0] = ww[1] = ww[2] = ww[3] = v;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int r = lane + 32 * j;
-                        ww[j] = (wsf && r < w_here) ? load_word(wsf + (long long)r * a.nkb, kb, w_words) : 0x7F7F7F7Fu;
-                    }
-                }
-            };
-            const int n_groups = g_last - g_first;
-            int i0 = (int)((mine ^ sfg) & 1u);    // first group of this tile that is this warp's
-            uint32_t wx[kXj], ww[4];
+            if (entered) {
+                if (!mm_tile<kPair>(a, start, before, t, lane, tl)) return false;
+                const int r0 = tl.w_row + 128 * (int)half;
+                const long long plane = (long long)tl.group * a.w_sf_rows;
+                if (a.w_sf) wsf = a.w_sf + (plane + (a.w_per_row ? r0 : r0 >> 7)) * a.nkb;
+                if (a.x_sf) xsf = a.x_sf + (long long)tl.x_row * a.x_sf_stride;
+                w_here = a.cols - r0;
+                valid = tl.valid;
+            }
+            const int kb = (g_first + g) * 4;
             if (!waited) {
                 grid_wait();
                 waited = true;
             }
-            if (i0 < n_groups) load_group(g_first + i0, wx, ww);
-            for (int i = i0; i < n_groups; i += 2) {
-                const uint32_t gg = sfg + (uint32_t)i, slot = gg % (uint32_t)a.sf_slots, par = (gg / (uint32_t)a.sf_slots) & 1u;
-                bool ok = true;
-                if (lane == 0) ok = mbar_wait(&S->sf_empty[slot], par ^ 1u, wait_ns, abort_flag);
-                ok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;
-                if (!ok) { dead = true; break; }
-                uint4* dst = reinterpret_cast<uint4*>(sf_tiles + slot * kSfSlotBytes);
-                dst[lane] = make_uint4(ww[0], ww[1], ww[2], ww[3]);
 #pragma unroll
-                for (int j = 0; j < kXTiles; ++j) dst[32 * (j + 1) + lane] = make_uint4(wx[4 * j], wx[4 * j + 1], wx[4 * j + 2], wx[4 * j + 3]);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (i + 2 < n_groups) load_group(g_first + i + 2, wx, ww);   // in flight while the copy is issued and the slot awaited
-                if (lane == 0) {
-                    const uint32_t tsf = tmem_base + (uint32_t)a.sf_col + slot * kSfSlotCols;
-                    const uint64_t sfdesc = umma_smem_desc_sf(smem_u32(dst));
-                    if constexpr (kPair) {
-                        if (leader) {   // one copy serves both CTAs: the partner's tile must be in place
-                            ok = wait_bar(&S->sf_peer[slot], par);
-                            if (ok) {
-                                tc_fence_after();
+            for (int j = 0; j < kXj; ++j) {
+                const int r = lane + 32 * j;
+                load_word(wx[j], xsf + (long long)r * a.x_sf_stride, xsf && r < valid, kb, x_words);
+            }
+            if (!a.w_per_row) {   // a 128 x 128 block: one word for all rows
+                load_word(ww[0], wsf, wsf && w_here > 0, kb, w_words);
+            } else {
 #pragma unroll
-                                for (int j = 0; j < kSfTiles; ++j) utccp_32x128b_warpx4_pair(tsf + 4 * j, sfdesc + (j * kMmSfTile >> 4));
-                                umma_commit_pair(mapa_u32(smem_u32(&S->sf_full[slot]), first));
-                            }
-                        } else {
-                            arrive_leader(&S->sf_peer[slot]);
-                        }
-                    } else {
+                for (int j = 0; j < 4; ++j) {
+                    const int r = lane + 32 * j;
+                    load_word(ww[j], wsf + (long long)r * a.nkb, wsf && r < w_here, kb, w_words);
+                }
+            }
+            g += 2;
+            return true;
+        };
+        bool dead = false, loaded = load_next();
+        uint32_t slot = mine, par = 0;   // sf_slots is at least two
+        while (loaded) {
+            bool ok = true;
+            if (lane == 0) ok = mbar_wait(&S->sf_empty[slot], par ^ 1u, wait_ns, abort_flag);
+            ok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;
+            if (!ok) { dead = true; break; }
+            uint4* dst = reinterpret_cast<uint4*>(sf_tiles + slot * kSfSlotBytes);
+            dst[lane] = a.w_per_row ? make_uint4(ww[0], ww[1], ww[2], ww[3]) : make_uint4(ww[0], ww[0], ww[0], ww[0]);
+#pragma unroll
+            for (int j = 0; j < kXTiles; ++j) dst[32 * (j + 1) + lane] = make_uint4(wx[4 * j], wx[4 * j + 1], wx[4 * j + 2], wx[4 * j + 3]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            // the arrival is a release and would wait for loads under way, so it comes before them
+            if (kPair && !leader && lane == 0) arrive_leader(&S->sf_peer[slot]);
+            loaded = load_next();   // in flight while the copy is issued and the slot awaited
+            if (leader && lane == 0) {
+                const uint32_t tsf = tmem_base + (uint32_t)a.sf_col + slot * kSfSlotCols;
+                const uint64_t sfdesc = umma_smem_desc_sf(smem_u32(dst));
+                if constexpr (kPair) {   // one copy serves both CTAs: the partner's tile must be in place
+                    ok = wait_bar(&S->sf_peer[slot], par);
+                    if (ok) {
                         tc_fence_after();
 #pragma unroll
-                        for (int j = 0; j < kSfTiles; ++j) utccp_32x128b_warpx4(tsf + 4 * j, sfdesc + (j * kMmSfTile >> 4));
-                        umma_commit(&S->sf_full[slot]);
+                        for (int j = 0; j < kSfTiles; ++j) utccp_32x128b_warpx4_pair(tsf + 4 * j, sfdesc + (j * kMmSfTile >> 4));
+                        umma_commit_pair(mapa_u32(smem_u32(&S->sf_full[slot]), first));
                     }
+                } else {
+                    tc_fence_after();
+#pragma unroll
+                    for (int j = 0; j < kSfTiles; ++j) utccp_32x128b_warpx4(tsf + 4 * j, sfdesc + (j * kMmSfTile >> 4));
+                    umma_commit(&S->sf_full[slot]);
                 }
-                ok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;
-                if (!ok) { dead = true; break; }
             }
-            sfg += (uint32_t)n_groups;
+            ok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;
+            if (!ok) { dead = true; break; }
+            slot += 2;
+            if (slot >= (uint32_t)a.sf_slots) { slot -= (uint32_t)a.sf_slots; par ^= 1u; }
         }
         if (dead && lane == 0) mm_raise(S, MXK_DEV_TIMEOUT_PIPE);
     } else {
@@ -488,7 +528,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
         grid_wait();   // kernels before this one may still read what is written here
         uint32_t it = 0;
         bool dead = false;
-        for (int t = unit; mm_tile<kPair>(a, start, before, t, tl); t += n_units, ++it) {
+        for (int t = unit; mm_tile<kPair>(a, start, before, t, lane, tl); t += n_units, ++it) {
             const uint32_t buf = it & 1u, use = it >> 1;
             bool ok = true;
             if (lane == 0) ok = wait_bar(&S->acc_full[buf], use & 1u);
@@ -524,7 +564,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                 for (int c = part; c < n_chunks; c += 2) push(c);
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) arrive_leader(&S->acc_empty[buf]);
+                if (lane == 0) drained(&S->acc_empty[buf]);
             } else {
                 const int col = tl.w_row + 128 * (int)half + q * 32 + lane;
                 uint32_t v[16];
@@ -548,7 +588,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) arrive_leader(&S->acc_empty[buf]);
+                if (lane == 0) drained(&S->acc_empty[buf]);
             }
             if (a.splits > 1) {
                 ok = mbar_wait_cluster(&S->red_full, it & 1u, wait_ns, abort_flag);
