@@ -87,48 +87,35 @@ __device__ __forceinline__ uint32_t mm_barrier_count(int i, uint32_t ctas, uint3
 static_assert(offsetof(MmSmem, tmem_base) == kMmBarriers * sizeof(uint64_t), "barriers first, without gaps");
 
 struct MmTile {
-    int group = 0, w_row, x_row, bt, valid;    // w_row: first weight row inside the group; x_row, bt: rows of x
-    int n = -1, row0, tile0, tt, per;          // of the group: rows, first row, first tile, tiles over the rows, rows of a tile
+    int group, w_row, x_row, bt, valid;    // w_row: first weight row inside the group; x_row, bt: rows of x
 };
 
 // status word of the products on this device: 0, or the first wait that expired
 __device__ int g_mm_status = 0;
 
-// Tile t of the list, found by a whole warp from the tile before it (t only grows): groups in order; inside a group the
-// operand with fewer rows turns fastest, so that the other one is read from memory once while the first stays in L2.  Every
-// role does this between two tiles, so it is kept short: one round trip to shared memory per 32 groups that are passed, and what
-// belongs to the group is computed once (a binary search and two divisions per tile: 800 clocks under load).
+// Tile t of the list: groups in order; inside a group the operand with fewer rows turns fastest,
+// so that the other one is read from memory once while the first stays in L2.
 template <bool kPair>
-__device__ __forceinline__ bool mm_tile(const MmArgs& a, const int* start, const int* before, int t, int lane, MmTile& o) {
+__device__ __forceinline__ bool mm_tile(const MmArgs& a, const int* start, const int* before, int t, MmTile& o) {
     if (t >= before[a.experts]) return false;
-    int lo = o.group;   // the last group with before[g] <= t; empty groups share a value with their successor
-    for (;;) {
-        const int e = lo + 1 + lane;
-        const unsigned passed = __ballot_sync(0xFFFFFFFFu, e < a.experts && before[e] <= t);
-        lo += __popc(passed);
-        if (passed != 0xFFFFFFFFu) break;
+    int lo = 0, hi = a.experts;   // last group with before[g] <= t; empty groups share a value with their successor
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (before[mid] <= t) lo = mid; else hi = mid;
     }
-    if (lo != o.group || o.n < 0) {
-        o.group = lo;
-        o.row0 = start[lo];
-        o.tile0 = before[lo];
-        o.n = o.per = start[lo + 1] - o.row0;
-        o.tt = 1;
-        if (o.n > a.bt_max) {
-            o.tt = a.fbt.div(o.n + a.bt_max - 1);
-            o.per = (o.n + o.tt - 1) / o.tt;
-        }
-        o.bt = (o.per + 15) & ~15;   // the group's rows spread evenly over its tiles
-    }
-    int xt = 0, wt = t - o.tile0;
-    if (o.tt > 1) {
-        const int i = wt;
-        if (o.n <= a.cols) { wt = i / o.tt; xt = i - wt * o.tt; }
+    const int n = start[lo + 1] - start[lo], i = t - before[lo];
+    int xt = 0, wt = i, per = n;
+    if (n > a.bt_max) {
+        const int tt = a.fbt.div(n + a.bt_max - 1);
+        if (n <= a.cols) { wt = i / tt; xt = i - wt * tt; }
         else { xt = a.fnt.div(i); wt = i - xt * a.n_tiles; }
+        per = (n + tt - 1) / tt;
     }
+    o.group = lo;
+    o.bt = (per + 15) & ~15;   // the group's rows spread evenly over its tiles
     o.w_row = wt * (kPair ? 256 : 128);
-    o.x_row = o.row0 + xt * o.bt;
-    o.valid = min(o.bt, o.n - xt * o.bt);
+    o.x_row = start[lo] + xt * o.bt;
+    o.valid = min(o.bt, n - xt * o.bt);
     return true;
 }
 
@@ -291,11 +278,11 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
 
     if (warp == 0) {
         // --------------------------------------------------------------- TMA producer
-        uint32_t stage = 0, phase = 0;
-        unsigned long long issued = 0;
-        bool dead = false, waited = false;
-        for (int t = unit; mm_tile<kPair>(a, start, before, t, lane, tl); t += n_units) {
-            if (lane == 0) {
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            unsigned long long issued = 0;
+            bool dead = false, waited = false;
+            for (int t = unit; !dead && mm_tile<kPair>(a, start, before, t, tl); t += n_units) {
                 // rows of all experts lie behind one another in the weight map; a tile that runs past its
                 // expert's last row reads the next expert's, and those output columns are not stored
                 const int w_row = (int)((long long)tl.group * a.cols) + tl.w_row + 128 * (int)half;
@@ -331,9 +318,6 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                     if (++stage == (uint32_t)a.n_stages) { stage = 0; phase ^= 1; }
                 }
             }
-            if (__any_sync(0xFFFFFFFFu, dead ? 1 : 0)) break;
-        }
-        if (lane == 0) {
             if (dead || *abort_flag) {
                 if (dead) mm_raise(S, MXK_DEV_TIMEOUT_PIPE);
                 // nothing may still be on its way into this shared memory when the CTA ends
@@ -368,7 +352,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                 if constexpr (kPair) umma_commit_pair_at(smem_u32(bar), first);
                 else umma_commit(bar);
             };
-            for (int t = unit; !dead && mm_tile<kPair>(a, start, before, t, lane, tl); t += n_units, ++it) {
+            for (int t = unit; !dead && mm_tile<kPair>(a, start, before, t, tl); t += n_units, ++it) {
                 const uint32_t idesc0 = umma_idesc_mx_e4m3(kPair ? 256 : 128, tl.bt, 0, 0) | a.formats;
                 const uint32_t buf = it & 1u, use = it >> 1;
                 const uint32_t tacc = tmem_base + buf * (uint32_t)a.bt_max;
@@ -447,7 +431,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                 entered = true;
             }
             if (entered) {
-                if (!mm_tile<kPair>(a, start, before, t, lane, tl)) return false;
+                if (!mm_tile<kPair>(a, start, before, t, tl)) return false;
                 const int r0 = tl.w_row + 128 * (int)half;
                 const long long plane = (long long)tl.group * a.w_sf_rows;
                 if (a.w_sf) wsf = a.w_sf + (plane + (a.w_per_row ? r0 : r0 >> 7)) * a.nkb;
@@ -528,7 +512,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
         grid_wait();   // kernels before this one may still read what is written here
         uint32_t it = 0;
         bool dead = false;
-        for (int t = unit; mm_tile<kPair>(a, start, before, t, lane, tl); t += n_units, ++it) {
+        for (int t = unit; mm_tile<kPair>(a, start, before, t, tl); t += n_units, ++it) {
             const uint32_t buf = it & 1u, use = it >> 1;
             bool ok = true;
             if (lane == 0) ok = wait_bar(&S->acc_full[buf], use & 1u);
