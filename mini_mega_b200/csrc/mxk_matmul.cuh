@@ -25,10 +25,11 @@
 // of one hides under the MMAs of the next.  (Both as the halves of one tile of 448 rows were slower, although a
 // quarter fewer bytes cross L2: MMAs that alternate between two accumulators ran at 75 % of the pipe.)
 //
-// What bounds it: many rows, the tensor pipe at the clock that the 1 kW cap leaves (4096 x 4096 x 7168: 97 us = 2.48
-// PFLOP/s in a burst, pipe 82 - 92 % busy at 1.55 - 1.6 GHz; 119 us in a loop of seconds); few rows, the weights'
-// stream (32 groups of 4 rows x 4096 x 6144: 121 us = 6.7 TB/s); the smallest calls, a chain of round trips of
-// some 5 us that starts under the predecessor's end (programmatic launch).
+// What bounds it: many rows, the tensor pipe at the clock that the 1 kW cap leaves (4096 x 4096 x 7168: 93 us = 2.57
+// PFLOP/s in a burst, 112 us in a loop of seconds, at 1.55 - 1.6 GHz); few rows, the weights' stream (32 groups of 4
+// rows x 4096 x 6144: 121 us = 6.7 TB/s); the smallest calls, a chain of round trips of some 5 us that starts under
+// the predecessor's end (programmatic launch).  Rows of an operand that are no multiple of 32 bytes apart cost a
+// third: half of the tile loads' rows then straddle a sector (2043 x 1111 x 4016: 17.6 us, at depth 4000 14.5, 4096 13.4).
 //
 // Few tiles (small batches): the K extent is split over the CTAs of a cluster, the partial tiles
 // are exchanged through distributed shared memory and added in the order of the splits, so results
@@ -143,7 +144,8 @@ __device__ __forceinline__ void ld_if(uint32_t& v, const void* p, bool has) {
     asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %2, 0;\n@q ld.global.b32 %0, [%1];\n}\n" : "+r"(v) : "l"(p), "r"((int)has));
 }
 // An arrival, here or in another CTA of the cluster, that orders no memory: what it reports are reads of tensor memory,
-// which tcgen05.wait and tcgen05.fence have ordered before it.
+// which tcgen05.wait and tcgen05.fence have ordered before it.  As a release it would wait for the warp's stores of the
+// result, some 1700 clocks a tile (32 groups of 300 rows x 2048 x 512: 33 us with it, 26 without).
 __device__ __forceinline__ void mbar_arrive_relaxed(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -507,7 +509,8 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
         // 16 accumulator columns (rows of x), and stores each row's 32 columns as one 64-byte piece straight from
         // registers.  Beside the running MMAs that was faster than fewer, wider stores: 4096 x 4096 x 1024
         // 25.4 us like this, 27.6 with chunks turned round in shared memory and 16 bytes a lane, 32.0 with shuffles
-        // and 4 bytes (rows off every alignment, 4095 columns: 28.0, 40.6, 29.0).
+        // and 4 bytes (rows off every alignment, 4095 columns: 28.0, 40.6, 29.0; all before the arrival behind them
+        // stopped waiting for the stores, 23.9 like this since).
         const int q = warp & 3, part = (warp - kMmFirstEpi) >> 2;
         grid_wait();   // kernels before this one may still read what is written here
         uint32_t it = 0;

@@ -4,7 +4,7 @@
 // The layer's own calls go through ctypes: one of them is 150 us and more of GPU work.  An operator
 // can be a few microseconds of it, and the same binding in Python (argument checks, allocation,
 // stream look-up, ctypes) took 17 to 19 us of host time per call and 130 us for a forward and backward
-// pass; here it is 4 to 6 us.  Checks raise before anything touches a device, so they hold on a host
+// pass; here it is 4 to 5 us and 49 to 58 (torch's own product: 47 to 51).  Checks raise before anything touches a device, so they hold on a host
 // without one.  All compute is in libmxk_b200.so, reached through its C ABI.
 // ============================================================================
 #include <ATen/ATen.h>
