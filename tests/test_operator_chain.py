@@ -81,6 +81,55 @@ def test_capture_of_the_whole_run_follows_its_inputs():
         assert torch.equal(held, _apart(x, x_sf, idx, weights, l1, l2, 8))
 
 
+def test_branches_that_join_and_copies_in_a_graph():
+    """Kernels behind copies from the host, on three streams, and with two predecessors: eager and captured."""
+    gen = torch.Generator().manual_seed(9)
+    tokens, hidden, topk, experts, cols = 300, 512, 8, 16, 384
+    host_idx = torch.randint(0, experts, (tokens, topk), generator=gen).pin_memory()
+    host_x = torch.randint(-8, 9, (tokens, hidden), generator=gen).to(torch.bfloat16).pin_memory()
+    q = torch.randint(-3, 4, (tokens, hidden), generator=gen).float().cuda().to(torch.float8_e4m3fn)
+    w = torch.randint(-3, 4, (cols, hidden), generator=gen).float().cuda().to(torch.float8_e4m3fn)
+    all_w = w.expand(experts, cols, hidden).contiguous()
+    idx, x = torch.zeros((tokens, topk), dtype=torch.int64, device="cuda"), torch.zeros((tokens, hidden), dtype=torch.bfloat16, device="cuda")
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def run():
+        here = torch.cuda.current_stream()
+        idx.copy_(host_idx, non_blocking=True)
+        plan = mm.plan_tokens_by_expert(idx, experts)
+        for s in streams:
+            s.wait_stream(here)
+        with torch.cuda.stream(streams[0]):
+            x.copy_(host_x, non_blocking=True)
+            dense = mm.fp8_matmul(q, w)
+        with torch.cuda.stream(streams[1]):
+            grouped = mm.fp8_grouped_matmul(mm.sort_tokens_by_expert(q, plan), all_w, plan.offsets)
+        here.wait_stream(streams[0])
+        rows = mm.sort_tokens_by_expert(x, plan)
+        here.wait_stream(streams[1])
+        return dense, rows, mm.unsort_tokens_by_expert(rows, plan), mm.unsort_tokens_by_expert(grouped, plan)
+
+    product = (q.double() @ w.double().t()).to(torch.bfloat16)
+    order = torch.sort(host_idx.reshape(-1), stable=True).indices // topk
+    want = (product, host_x[order].cuda(), (host_x.float() * topk).to(torch.bfloat16).cuda(), (product.float() * topk).to(torch.bfloat16))
+    run()
+    torch.cuda.synchronize()
+    for got, w_ in zip(run(), want):
+        torch.cuda.synchronize()
+        assert torch.equal(got, w_)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run()
+    for _ in range(10):
+        for t in (idx, x, *held):
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, w_ in zip(held, want):
+            assert torch.equal(got, w_)
+    assert mm.matmul_status() == 0
+
+
 def test_inference_mode_and_sign_flag_views():
     """Tables, rows and results made in inference mode; inputs that are views with their sign in a flag."""
     case = orc.gen_case(1, 8, 2, 512, 256, 33, seed=5, routing="logits", scaled=True)
