@@ -11,9 +11,12 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <c10/core/AutogradState.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cstring>
@@ -54,6 +57,17 @@ void same_device(const char* fn, const Tensor& first, std::initializer_list<cons
     MXK_VALUE(d.is_cuda(), fn, " runs on CUDA tensors only, got ", d.str());
 }
 
+// The calls pass the dispatcher by, so whoever follows a computation through it sees a fresh result without a past: a
+// tangent would be lost and a tracer would store the result as a constant, both without a word.  They are refused.
+void not_followed(const char* fn, std::initializer_list<const Tensor*> inputs) {
+    if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY))
+        throw std::runtime_error(std::string(fn) + ": cannot be traced");
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor* t : inputs)
+        if (t && t->defined() && t->_fw_grad(0).defined())
+            throw std::runtime_error(std::string(fn) + ": has no forward-mode derivative, got an input with a tangent");
+}
+
 Tensor rows_contiguous(const Tensor& t) {
     if (t.is_neg()) return t.resolve_neg().contiguous();   // a view that carries its sign in a flag
     return t.stride(1) == 1 || t.size(1) == 1 ? t : t.contiguous();
@@ -82,6 +96,7 @@ int type_code(at::ScalarType t) {
 
 std::tuple<Tensor, Tensor, Tensor> plan_tokens(const Tensor& topk_idx, int64_t num_experts, int64_t first_expert) {
     const char* fn = "plan_tokens_by_expert";
+    not_followed(fn, {});
     MXK_TYPE(topk_idx.scalar_type() == at::kLong || topk_idx.scalar_type() == at::kInt, fn, ": topk_idx must be an int64 or int32 tensor");
     MXK_VALUE(topk_idx.dim() == 2 && topk_idx.size(1) >= 1 && topk_idx.size(1) <= kMaxTopk, fn, ": topk_idx must be [tokens, topk] with 1 <= topk <= ", kMaxTopk, ", got ", topk_idx.sizes());
     MXK_VALUE(num_experts >= 1 && num_experts <= kMaxExperts, fn, ": num_experts must be in [1, ", kMaxExperts, "], got ", num_experts);
@@ -165,6 +180,7 @@ struct SortFunction : torch::autograd::Function<SortFunction> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
+        not_followed("sort_tokens_by_expert (backward)", {&grads[0]});
         return {unsort_differentiable(grads[0], Tensor(), saved[0], saved[1]), Tensor(), Tensor()};
     }
 };
@@ -176,6 +192,7 @@ struct SumFunction : torch::autograd::Function<SumFunction> {   // unsort withou
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
+        not_followed("unsort_tokens_by_expert (backward)", {&grads[0]});
         return {sort_differentiable(grads[0], saved[0], saved[1]), Tensor(), Tensor()};
     }
 };
@@ -190,6 +207,7 @@ struct UnsortFunction : torch::autograd::Function<UnsortFunction> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const Tensor &weights_in = saved[1], &row_of_pair = saved[2], &offsets = saved[3];
+        not_followed("unsort_tokens_by_expert (backward)", {&grads[0]});
         if (at::GradMode::is_enabled()) throw std::runtime_error("unsort_tokens_by_expert: the weighted sum has no second derivative (create_graph)");
         const c10::cuda::CUDAGuard guard(grads[0].device());
         const int64_t tokens = row_of_pair.size(0), topk = row_of_pair.size(1);
@@ -224,6 +242,7 @@ bool under_capture() { return c10::cuda::currentStreamCaptureStatusMayInitCtx() 
 
 py::object sort_tokens(const Tensor& x, const Tensor& row_of_pair, const Tensor& pair_of_row, const Tensor& offsets, const MaybeTensor& x_sf) {
     const char* fn = "sort_tokens_by_expert";
+    not_followed(fn, {&x});
     check_plan(fn, row_of_pair, pair_of_row, offsets);
     MXK_TYPE(type_code(x.scalar_type()) >= 0 || byte_type(x.scalar_type()), fn, ": x must be a bf16, fp16, fp32 or 8-bit tensor");
     MXK_VALUE(x.dim() == 2 && x.size(0) == row_of_pair.size(0) && x.size(1) >= 1 && x.size(1) <= kMaxHidden, fn, ": x must be [", row_of_pair.size(0), ", hidden], got ", x.sizes());
@@ -246,6 +265,7 @@ py::object sort_tokens(const Tensor& x, const Tensor& row_of_pair, const Tensor&
 
 Tensor unsort_tokens(const Tensor& rows, const Tensor& row_of_pair, const Tensor& pair_of_row, const Tensor& offsets, const MaybeTensor& topk_weights) {
     const char* fn = "unsort_tokens_by_expert";
+    not_followed(fn, {&rows, topk_weights ? &*topk_weights : nullptr});
     check_plan(fn, row_of_pair, pair_of_row, offsets);
     MXK_TYPE(type_code(rows.scalar_type()) >= 0, fn, ": rows must be a bf16, fp16 or fp32 tensor");
     MXK_VALUE(rows.dim() == 2 && rows.size(0) == row_of_pair.numel() && rows.size(1) >= 1 && rows.size(1) <= kMaxHidden, fn, ": rows must be [", row_of_pair.numel(), ", hidden], got ", rows.sizes());
@@ -270,6 +290,7 @@ int format_code(at::ScalarType t) {
 
 Tensor matmul(const char* fn, const Tensor& x, const MaybeTensor& x_sf, const Tensor& w, const MaybeTensor& w_sf, const MaybeTensor& offsets, const MaybeTensor& out_in) {
     const int64_t w_dim = offsets ? 3 : 2;
+    not_followed(fn, {&x, &w, out_in ? &*out_in : nullptr});
     MXK_TYPE(format_code(x.scalar_type()) >= 0, fn, ": x must be a float8_e4m3fn, float8_e5m2 (or raw uint8 E4M3) tensor");
     MXK_TYPE(format_code(w.scalar_type()) >= 0, fn, ": w must be a float8_e4m3fn, float8_e5m2 (or raw uint8 E4M3) tensor");
     MXK_TYPE(!at::GradMode::is_enabled() || !(x.requires_grad() || w.requires_grad()), fn, ": has no gradient: detach the operands, or call it under no_grad");

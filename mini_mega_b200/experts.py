@@ -10,7 +10,8 @@ something of their own between them, and for training::
 
 Pair ``p = token * topk + j``; inside an expert the rows lie in ascending pair order (the order of the layer's own
 dispatch), so a plan, and everything computed with it, is the same on every run.  Calls run on the current stream
-of the tensors' device, allocate only their results and can be captured into CUDA graphs.
+of the tensors' device, allocate only their results and can be captured into CUDA graphs.  There is no forward-mode
+derivative: inputs with a tangent are refused, and so are calls under a tracer (``torch.jit.trace``, ``make_fx``).
 """
 from __future__ import annotations
 

@@ -23,7 +23,8 @@ def fp8_matmul(x: Operand, w: Operand, out: Optional[torch.Tensor] = None) -> to
     ``[cols, ceil(depth / 128)]`` (per row: the form in which both factors are activations, such as a weight gradient
     from its two factors quantised along the tokens).  ``depth`` is a multiple of 16; rows of both operands are 16-byte
     aligned and may be apart.  Scale byte e stands for ``2**(e - 127)``; 255 is NaN.  There is no
-    gradient: operands that ask for one are refused while gradients are recorded."""
+    gradient: operands that ask for one are refused while gradients are recorded, operands with a forward-mode tangent and
+    calls under a tracer (``torch.jit.trace``, ``make_fx``) always."""
     xd, xs = x if isinstance(x, tuple) else (x, None)
     wd, ws = w if isinstance(w, tuple) else (w, None)
     return _lib.ops().fp8_matmul(xd, xs, wd, ws, out)

@@ -1,0 +1,90 @@
+"""The operators beside the layer at their edges: calls whose result would be wrong without a word are refused, and
+sizes, tables and cuts that the plain tests do not reach.  Bounds as in test_matmul.py and test_expert_rows.py.
+"""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+from torch.fx.experimental.proxy_tensor import make_fx
+
+import mini_mega_b200 as mm
+from mini_mega_b200 import _lib
+
+E4 = torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module", autouse=True)
+def built():
+    _lib.build()
+
+
+def _plan(device="cpu"):
+    """4 tokens x 2 pairs on 3 experts, all of them on expert 0."""
+    place = torch.arange(8, dtype=torch.int32, device=device)
+    return mm.ExpertPlan(place.view(4, 2), place.clone(), torch.tensor([0, 8, 8, 8], dtype=torch.int32, device=device))
+
+
+def _dual(t):
+    return fwAD.make_dual(t, torch.ones_like(t))
+
+
+# ------------------------------------------------- tangents and tracers, which a result made here would lose
+def _followed(device):
+    z = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype, device=device)   # noqa: E731
+    plan, off = _plan(device), torch.zeros(4, dtype=torch.int32, device=device)
+    out = lambda rows, cols: z(rows, cols, dtype=torch.bfloat16)   # noqa: E731
+    return {
+        "sort": (lambda t: mm.sort_tokens_by_expert(t, plan), z(4, 8)),
+        "sort that asks for a gradient": (lambda t: mm.sort_tokens_by_expert(t.requires_grad_(), plan), z(4, 8)),
+        "sort with scales": (lambda t: mm.sort_tokens_by_expert(t, plan, z(4, 1, dtype=torch.uint8))[0], z(4, 128, dtype=E4)),
+        "unsort, rows": (lambda t: mm.unsort_tokens_by_expert(t, plan), z(8, 8)),
+        "unsort with weights, rows": (lambda t: mm.unsort_tokens_by_expert(t, plan, z(4, 2)), z(8, 8)),
+        "unsort, weights": (lambda t: mm.unsort_tokens_by_expert(z(8, 8), plan, t), z(4, 2)),
+        "product, x": (lambda t: mm.fp8_matmul(t, z(8, 128, dtype=E4)), z(4, 128, dtype=E4)),
+        "product, w": (lambda t: mm.fp8_matmul(z(4, 128, dtype=E4), t), z(8, 128, dtype=E4)),
+        "product, out": (lambda t: mm.fp8_matmul(z(4, 128, dtype=E4), z(8, 128, dtype=E4), out=t), out(4, 8)),
+        "grouped product, x": (lambda t: mm.fp8_grouped_matmul(t, z(3, 8, 128, dtype=E4), off), z(4, 128, dtype=E4)),
+    }
+
+
+@pytest.mark.parametrize("name", list(_followed("cpu")))
+def test_a_tangent_is_refused_not_dropped(name):
+    call, t = _followed("cpu")[name]
+    with fwAD.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        call(_dual(t))
+    with fwAD.dual_level(), torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):   # torch carries tangents on there
+        call(_dual(t))
+    with fwAD.dual_level(), fwAD._set_fwd_grad_enabled(False), pytest.raises(ValueError, match="CUDA"):   # nothing to lose
+        call(_dual(t))
+
+
+@pytest.mark.parametrize("name", list(_followed("cpu")))
+def test_a_tracer_is_refused_not_given_a_constant(name):
+    call, t = _followed("cpu")[name]
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(call, (t,))
+    with pytest.raises(RuntimeError, match="traced"):
+        make_fx(call)(t)
+
+
+def test_a_plan_is_not_traced():
+    idx = torch.zeros((4, 2), dtype=torch.int64)
+    for trace in (lambda f: torch.jit.trace(f, (idx,)), lambda f: make_fx(f)(idx)):
+        with pytest.raises(RuntimeError, match="traced"):
+            trace(lambda i: mm.plan_tokens_by_expert(i, 3))
+
+
+@pytest.mark.gpu
+def test_a_tangent_of_an_incoming_gradient_is_refused():
+    plan, w = _plan("cuda"), torch.rand((4, 2), device="cuda")
+    x, rows = torch.randn((4, 8), device="cuda", requires_grad=True), torch.randn((8, 8), device="cuda", requires_grad=True)
+    for y, leaf in ((mm.sort_tokens_by_expert(x, plan), x), (mm.unsort_tokens_by_expert(rows, plan), rows),
+                    (mm.unsort_tokens_by_expert(rows, plan, w), rows)):
+        dy = torch.ones_like(y)
+        with fwAD.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, leaf, _dual(dy), retain_graph=True)
+        torch.autograd.grad(y, leaf, dy)
+    for name, (call, t) in _followed("cuda").items():
+        with fwAD.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            call(_dual(t))
+        with fwAD.dual_level():   # a level without tangents
+            call(t)
