@@ -432,6 +432,7 @@ typedef struct MxkMatmulArgs {
     int32_t w_sf_per_row;
     int32_t zero_tail;         /* grouped: clear out rows of no expert (0: they are left alone)     */
     int32_t max_spins;         /* bound of every device wait in units of 250 ns, at least 8000000 (2 s); 0 => 2 s.
+                                * It counts from the end of the kernels in front of the product in its stream.
                                 * 4 us per 128 columns of depth come on top: a wait that expires while the
                                 * product is healthy would leave with its copies and MMAs under way    */
 } MxkMatmulArgs;

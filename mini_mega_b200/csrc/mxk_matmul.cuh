@@ -189,8 +189,9 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
 
     // Start-up, kept short because it is a fifth of a small product: warp 0 initialises the barriers, builds the
     // group table and goes on to its first loads without waiting for the others; warp 1 meanwhile allocates TMEM.
-    // Every role waits for the kernels before this one (grid_wait) where it first touches memory and not earlier, so that
-    // its way there, instruction fetches included, lies under their end.
+    // Every role waits for the kernels before this one (grid_wait) where it first touches memory or first waits for one that
+    // does, and not earlier, so that its way there, instruction fetches included, lies under their end.  Not later either: a
+    // bounded wait that began under a long kernel (a collective behind a late rank) would run out in a healthy product.
     grid_let_next_begin();
     if (clustered && warp != 0) cluster_arrive();
     if (warp == 0) {
@@ -354,6 +355,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                 if constexpr (kPair) umma_commit_pair_at(smem_u32(bar), first);
                 else umma_commit(bar);
             };
+            grid_wait();   // nothing arrives before the loads do: the bounded waits shall not count the kernels before this one
             for (int t = unit; !dead && mm_tile<kPair>(a, start, before, t, tl); t += n_units, ++it) {
                 const uint32_t idesc0 = umma_idesc_mx_e4m3(kPair ? 256 : 128, tl.bt, 0, 0) | a.formats;
                 const uint32_t buf = it & 1u, use = it >> 1;

@@ -229,7 +229,8 @@ MmShape mm_shape(int64_t rows, int64_t cols, int64_t depth, int64_t experts, boo
 }
 
 // A wait that expires ends its CTA, which must not happen while copies or MMAs of a healthy product are still on their
-// way into that CTA's memory: bounds below this are refused, and the longest wait (a tile's whole K loop) gets 4 us per
+// way into that CTA's memory: bounds below this are refused, no wait begins before the kernels in front have ended
+// (grid_wait in every role), and the longest wait (a tile's whole K loop) gets 4 us per
 // K block on top, more than ten times what one takes.
 constexpr int kMmLeastSpins = 8000000;
 

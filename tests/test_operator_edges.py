@@ -1,6 +1,9 @@
 """The operators beside the layer at their edges: calls whose result would be wrong without a word are refused, and
 sizes, tables and cuts that the plain tests do not reach.  Bounds as in test_matmul.py and test_expert_rows.py.
 """
+import os
+import re
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -88,3 +91,24 @@ def test_a_tangent_of_an_incoming_gradient_is_refused():
             call(_dual(t))
         with fwAD.dual_level():   # a level without tangents
             call(t)
+
+
+# --------------------------------------------------------- bounded waits and the kernels before a product
+def _product_roles():
+    """The text of every warp role of the product kernel, comments taken out."""
+    path = os.path.join(os.path.dirname(os.path.abspath(_lib.__file__)), "csrc", "mxk_matmul.cuh")
+    text = open(path).read()
+    text = text[text.index("void mm_body("):text.index("nobody leaves while a partner")]
+    parts = re.split(r"// -{20,} (TMA producer|MMA issuer|scale-tile builders|epilogue)\n", text)
+    return {name: re.sub(r"//.*", "", body) for name, body in zip(parts[1::2], parts[2::2])}
+
+
+@pytest.mark.parametrize("role, first", [("TMA producer", r"\bload\(sw"), ("MMA issuer", r"\bfor \(int t = unit"),
+                                         ("scale-tile builders", r"\bload_word\(wx"), ("epilogue", r"\bfor \(int t = unit")])
+def test_no_bounded_wait_of_a_product_begins_under_the_kernel_before_it(role, first):
+    """A product may begin while the kernel in front of it still runs, for however long that takes; its waits are bounded.
+    So each role has to pass grid_wait() ahead of its first load, or ahead of its first wait for somebody else's (the
+    producer and the builders first wait for slots that are free at the start).  Read from the source: showing it on a GPU
+    would take a kernel in front that runs for longer than the bound."""
+    body = _product_roles()[role]
+    assert "grid_wait();" in body and body.index("grid_wait();") < re.search(first, body).start()
