@@ -288,18 +288,24 @@ struct SortArgs {
     int sf_bytes, sf_vec;
 };
 
+// Scales wider than this are copied in parts, so that the count over a batch of tiles stays below 2^31.
+constexpr int kScalePart = 1 << 20;
+static_assert((long long)kRowBatch * kScalePart + kRowThreads < (1ll << 31), "32-bit index");
 template <int V>
 __device__ __forceinline__ void copy_scales(const SortArgs& a, const int* s_row, long long step0) {
     typedef typename VecOf<V>::T T;
-    const int n = a.sf_bytes / V, tiles = a.f.batch * a.f.tall;
-    for (int i = threadIdx.x; i < tiles * n; i += kRowThreads) {
-        const int q = i / n, at = i - q * n, step = q / a.f.tall;
-        const long long t = ((step0 + step) * gridDim.x + blockIdx.x) * a.f.tall + (q - step * a.f.tall);
-        if (t >= a.f.tokens) continue;
-        const T v = *reinterpret_cast<const T*>(a.x_sf + t * a.sf_stride + (long long)at * V);
-        for (int j = 0; j < a.f.topk; ++j) {
-            const int r = s_row[q * a.f.topk + j];
-            if (r >= 0) *reinterpret_cast<T*>(a.rows_sf + (long long)r * a.sf_bytes + (long long)at * V) = v;
+    const int all = a.sf_bytes / V, tiles = a.f.batch * a.f.tall;   // tiles <= kRowBatch
+    for (int first = 0; first < all; first += kScalePart) {
+        const int n = min(all - first, kScalePart);
+        for (int i = threadIdx.x; i < tiles * n; i += kRowThreads) {
+            const int q = i / n, at = first + i - q * n, step = q / a.f.tall;
+            const long long t = ((step0 + step) * gridDim.x + blockIdx.x) * a.f.tall + (q - step * a.f.tall);
+            if (t >= a.f.tokens) continue;
+            const T v = *reinterpret_cast<const T*>(a.x_sf + t * a.sf_stride + (long long)at * V);
+            for (int j = 0; j < a.f.topk; ++j) {
+                const int r = s_row[q * a.f.topk + j];
+                if (r >= 0) *reinterpret_cast<T*>(a.rows_sf + (long long)r * a.sf_bytes + (long long)at * V) = v;
+            }
         }
     }
 }

@@ -112,3 +112,23 @@ def test_no_bounded_wait_of_a_product_begins_under_the_kernel_before_it(role, fi
     would take a kernel in front that runs for longer than the bound."""
     body = _product_roles()[role]
     assert "grid_wait();" in body and body.index("grid_wait();") < re.search(first, body).start()
+
+
+# ------------------------------------------------------------------------------ sizes whose products pass 32 bits
+@pytest.mark.gpu
+@pytest.mark.parametrize("blocks", [(1 << 22) - 1, 1 << 22])
+def test_scales_of_very_wide_rows(blocks):
+    """600 rows of 2^22 bytes (one column of CTAs, which takes all 600 in one batch) with as many scale bytes, at an odd
+    width copied byte by byte: 600 (2^22 - 1) = 2.5e9 copies of one CTA are more than 31 bits count."""
+    tokens, hidden = 600, 1 << 22
+    g = torch.Generator(device="cuda").manual_seed(blocks)
+    idx = torch.randint(0, 3, (tokens, 1), device="cuda", generator=g)
+    x = torch.randint(0, 256, (tokens, hidden), device="cuda", generator=g, dtype=torch.uint8)
+    sf = torch.randint(0, 256, (tokens, blocks), device="cuda", generator=g, dtype=torch.uint8)
+    plan = mm.plan_tokens_by_expert(idx, 2)
+    rows, rows_sf = mm.sort_tokens_by_expert(x, plan, sf)
+    order, end = torch.sort(idx[:, 0], stable=True).indices, int((idx < 2).sum())
+    for first in range(0, end, 100):
+        at = order[first:min(first + 100, end)]
+        assert torch.equal(rows[first:first + len(at)], x[at]) and torch.equal(rows_sf[first:first + len(at)], sf[at])
+    assert not rows[end:].any() and not rows_sf[end:].any()
