@@ -400,6 +400,11 @@ int mxk_plan_tokens(const void* topk_idx, int32_t idx_bytes, int64_t idx_stride,
 int mxk_sort_tokens(const void* x, int64_t x_stride, int64_t row_bytes, const void* x_sf, int64_t sf_stride, int64_t sf_bytes,
                     int32_t tokens, int32_t topk, int32_t num_experts, const int32_t* row_of_pair, const int32_t* offsets,
                     void* rows, void* rows_sf, void* stream);
+/* The same with the plan's third table: cleared are all rows that no pair names, those behind offsets[num_experts] and
+ * those of pairs whose row_of_pair was set out of range after the plan (mxk_sort_tokens leaves the latter unwritten). */
+int mxk_sort_tokens_by_plan(const void* x, int64_t x_stride, int64_t row_bytes, const void* x_sf, int64_t sf_stride, int64_t sf_bytes,
+                            int32_t tokens, int32_t topk, int32_t num_experts, const int32_t* row_of_pair,
+                            const int32_t* pair_of_row, const int32_t* offsets, void* rows, void* rows_sf, void* stream);
 
 /* y[t] = sum over j of weights[t][j] * rows[row_of_pair[t][j]], j ascending, FP32, rounded once to the rows'
  * type (MXK_DTYPE_*); weights NULL: all one (the gradient of the sort).  Strides: bytes between rows, floats
@@ -413,6 +418,11 @@ int mxk_unsort_tokens_grad(const void* dy, int64_t dy_stride, const void* rows, 
                            const float* weights, int64_t weights_stride, int32_t tokens, int32_t topk, int32_t num_experts,
                            int32_t hidden, const int32_t* row_of_pair, const int32_t* offsets, void* drows, float* dweights,
                            void* stream);
+/* The same with the plan's third table: drows is 0 in all rows that no pair names, as in mxk_sort_tokens_by_plan. */
+int mxk_unsort_tokens_grad_by_plan(const void* dy, int64_t dy_stride, const void* rows, int64_t rows_stride, int32_t dtype,
+                                   const float* weights, int64_t weights_stride, int32_t tokens, int32_t topk, int32_t num_experts,
+                                   int32_t hidden, const int32_t* row_of_pair, const int32_t* pair_of_row, const int32_t* offsets,
+                                   void* drows, float* dweights, void* stream);
 
 /* out[m][n] = sum over k of x[m][k] 2^(x_sf[m][k / 128] - 127) * w[n][k] 2^(w_sf - 127), FP32 accumulation, bf16 out.
  * Dense (offsets NULL), or grouped: rows offsets[e] .. offsets[e + 1] of x and out meet the e-th weight matrix.

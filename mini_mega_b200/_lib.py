@@ -125,7 +125,8 @@ EXPORTS = [
     "mxk_static_scratch_bytes", "mxk_fill_weights", "mxk_fill_weights_e2m1", "mxk_e2m1_to_e4m3", "mxk_quantize_rows", "mxk_dump_kernel_resources", "mxk_read_status",
     "mxk_read_status_static", "mxk_rwk_ticks_off", "mxk_ticks_count", "mxk_set_ticks", "mxk_select_win",
     "mxk_group_ranks", "mxk_gs_schedule_member", "mxk_gs_schedule_member_hot", "mxk_gs_group_skewed", "mxk_lpt_assign", "mxk_gs_schedule_on_device",
-    "mxk_plan_tokens", "mxk_sort_tokens", "mxk_unsort_tokens", "mxk_unsort_tokens_grad", "mxk_fp8_matmul", "mxk_matmul_status",
+    "mxk_plan_tokens", "mxk_sort_tokens", "mxk_sort_tokens_by_plan", "mxk_unsort_tokens", "mxk_unsort_tokens_grad", "mxk_unsort_tokens_grad_by_plan",
+    "mxk_fp8_matmul", "mxk_matmul_status",
     "mxk_symm_alloc", "mxk_symm_free", "mxk_ipc_export", "mxk_ipc_import", "mxk_ipc_close",
 ]
 
@@ -177,8 +178,10 @@ def lib():
     vp, i32, i64 = C.c_void_p, C.c_int32, C.c_int64
     L.mxk_plan_tokens.argtypes = [vp, i32, i64, i32, i32, i32, i32, vp, vp, vp, vp]
     L.mxk_sort_tokens.argtypes = [vp, i64, i64, vp, i64, i64, i32, i32, i32, vp, vp, vp, vp, vp]
+    L.mxk_sort_tokens_by_plan.argtypes = [vp, i64, i64, vp, i64, i64, i32, i32, i32, vp, vp, vp, vp, vp, vp]
     L.mxk_unsort_tokens.argtypes = [vp, i32, i64, vp, i64, i32, i32, i32, vp, vp, vp]
     L.mxk_unsort_tokens_grad.argtypes = [vp, i64, vp, i64, i32, vp, i64, i32, i32, i32, i32, vp, vp, vp, vp, vp]
+    L.mxk_unsort_tokens_grad_by_plan.argtypes = [vp, i64, vp, i64, i32, vp, i64, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp]
     L.mxk_fp8_matmul.argtypes = [C.POINTER(MxkMatmulArgs), vp]
     L.mxk_matmul_status.argtypes = [C.POINTER(C.c_int32)]
     L.mxk_symm_alloc.argtypes = [C.POINTER(C.c_void_p), C.c_int64]

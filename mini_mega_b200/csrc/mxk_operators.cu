@@ -273,18 +273,25 @@ int mxk_plan_tokens(const void* topk_idx, int32_t idx_bytes, int64_t idx_stride,
 int mxk_sort_tokens(const void* x, int64_t x_stride, int64_t row_bytes, const void* x_sf, int64_t sf_stride, int64_t sf_bytes,
                     int32_t tokens, int32_t topk, int32_t num_experts, const int32_t* row_of_pair, const int32_t* offsets,
                     void* rows, void* rows_sf, void* stream) {
+    return mxk_sort_tokens_by_plan(x, x_stride, row_bytes, x_sf, sf_stride, sf_bytes, tokens, topk, num_experts, row_of_pair, nullptr,
+                                   offsets, rows, rows_sf, stream);
+}
+
+int mxk_sort_tokens_by_plan(const void* x, int64_t x_stride, int64_t row_bytes, const void* x_sf, int64_t sf_stride, int64_t sf_bytes,
+                            int32_t tokens, int32_t topk, int32_t num_experts, const int32_t* row_of_pair, const int32_t* pair_of_row,
+                            const int32_t* offsets, void* rows, void* rows_sf, void* stream) {
     if (bad_tables(tokens, topk) || num_experts < 1 || num_experts > kRowsMaxExperts || row_bytes < 1 || row_bytes > kMaxRowBytes || (x_sf && (sf_bytes < 1 || sf_bytes > (1 << 24))))
         return fail(MXK_ERR_BAD_ARG, "sort_tokens: sizes out of range");
     if (x_stride < 0 || sf_stride < 0) return fail(MXK_ERR_BAD_ARG, "sort_tokens: strides must not be negative");
     if (tokens == 0) return 0;
     if (!x || !rows || !row_of_pair || !offsets || (x_sf && !rows_sf)) return fail(MXK_ERR_BAD_ARG, "sort_tokens: pointers must be non-null");
-    if (!words(row_of_pair, offsets)) return fail(MXK_ERR_BAD_ARG, "sort_tokens: tables must be aligned to their element type");
+    if (!words(row_of_pair, pair_of_row, offsets)) return fail(MXK_ERR_BAD_ARG, "sort_tokens: tables must be aligned to their element type");
     const int vec = common_vec(addr(x) | addr(rows) | (uint64_t)x_stride | (uint64_t)row_bytes);
     SortArgs a;
     std::memset(&a, 0, sizeof(a));
     a.x = static_cast<const uint8_t*>(x); a.x_sf = static_cast<const uint8_t*>(x_sf);
     a.rows = static_cast<uint8_t*>(rows); a.rows_sf = static_cast<uint8_t*>(rows_sf);
-    a.end = offsets + num_experts;
+    a.tables = RowTables{row_of_pair, pair_of_row, offsets + num_experts, tokens * topk};
     a.x_stride = x_stride; a.sf_stride = sf_stride; a.sf_bytes = (int)sf_bytes;
     if (x_sf) {
         const int v = common_vec(addr(x_sf) | addr(rows_sf) | (uint64_t)sf_stride | (uint64_t)sf_bytes);
@@ -328,6 +335,14 @@ int mxk_unsort_tokens_grad(const void* dy, int64_t dy_stride, const void* rows, 
                            const float* weights, int64_t weights_stride, int32_t tokens, int32_t topk, int32_t num_experts,
                            int32_t hidden, const int32_t* row_of_pair, const int32_t* offsets, void* drows, float* dweights,
                            void* stream) {
+    return mxk_unsort_tokens_grad_by_plan(dy, dy_stride, rows, rows_stride, dtype, weights, weights_stride, tokens, topk, num_experts,
+                                          hidden, row_of_pair, nullptr, offsets, drows, dweights, stream);
+}
+
+int mxk_unsort_tokens_grad_by_plan(const void* dy, int64_t dy_stride, const void* rows, int64_t rows_stride, int32_t dtype,
+                                   const float* weights, int64_t weights_stride, int32_t tokens, int32_t topk, int32_t num_experts,
+                                   int32_t hidden, const int32_t* row_of_pair, const int32_t* pair_of_row, const int32_t* offsets,
+                                   void* drows, float* dweights, void* stream) {
     if (bad_tables(tokens, topk) || num_experts < 1 || num_experts > kRowsMaxExperts || hidden < 1 || hidden > kMaxRowBytes / 4 || dtype < MXK_DTYPE_BF16 || dtype > MXK_DTYPE_FP32)
         return fail(MXK_ERR_BAD_ARG, "unsort_tokens_grad: sizes or type out of range");
     if (dy_stride < 0 || rows_stride < 0 || weights_stride < 0) return fail(MXK_ERR_BAD_ARG, "unsort_tokens_grad: strides must not be negative");
@@ -336,14 +351,15 @@ int mxk_unsort_tokens_grad(const void* dy, int64_t dy_stride, const void* rows, 
     UnsortGradArgs a;
     std::memset(&a, 0, sizeof(a));
     a.dy = static_cast<const uint8_t*>(dy); a.rows = static_cast<const uint8_t*>(rows); a.w = weights;
-    a.drows = static_cast<uint8_t*>(drows); a.dw = dweights; a.row_of_pair = row_of_pair; a.end = offsets + num_experts;
+    a.drows = static_cast<uint8_t*>(drows); a.dw = dweights;
+    a.tables = RowTables{row_of_pair, pair_of_row, offsets + num_experts, tokens * topk};
     a.dy_stride = dy_stride; a.rows_stride = rows_stride; a.w_stride = weights_stride;
-    a.row_bytes = hidden * dtype_bytes(dtype); a.tokens = tokens; a.topk = topk; a.pairs = tokens * topk;
+    a.row_bytes = hidden * dtype_bytes(dtype); a.tokens = tokens; a.topk = topk;
     uint64_t bits = addr(dy) | (uint64_t)dy_stride | (uint64_t)a.row_bytes;
     if (drows) bits |= addr(drows);
     if (dweights) bits |= addr(rows) | (uint64_t)rows_stride;
     const int vec = common_vec(bits);
-    if (vec < dtype_bytes(dtype) || !words(weights, row_of_pair, offsets, dweights)) return fail(MXK_ERR_BAD_ARG, "unsort_tokens_grad: tensors must be aligned to their element type");
+    if (vec < dtype_bytes(dtype) || !words(weights, row_of_pair, pair_of_row, offsets, dweights)) return fail(MXK_ERR_BAD_ARG, "unsort_tokens_grad: tensors must be aligned to their element type");
     a.vecs = a.row_bytes / vec;
     a.team = 1;   // warps per token: as many as the row has columns for
     while (a.team < 8 && a.vecs > 32 * a.team) a.team *= 2;

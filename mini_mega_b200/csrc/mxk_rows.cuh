@@ -265,11 +265,40 @@ __device__ __forceinline__ void row_fetch(const RowFrame& f, const float* w, lon
 }
 
 template <int V>
-__device__ __forceinline__ void clear_row(uint8_t* row, int bytes) {
+__device__ __forceinline__ void clear_row(uint8_t* row, int bytes) {   // by one warp
     typedef typename VecOf<V>::T T;
     T z;
     memset(&z, 0, sizeof(z));
-    for (int i = threadIdx.x; i < bytes / V; i += kRowThreads) reinterpret_cast<T*>(row)[i] = z;
+    for (int i = threadIdx.x & 31; i < bytes / V; i += 32) reinterpret_cast<T*>(row)[i] = z;
+}
+
+// Rows that no pair names are cleared: those behind the last expert's, and those of pairs that the caller's tables drop
+// although a row was planned for them.  pair_of_row tells which: it names no pair, or one that is dropped now.  Without it
+// (null) only rows behind the end are cleared.  A row behind the end counts as named where the two tables agree on it.
+struct RowTables {
+    const int* row_of_pair;
+    const int* pair_of_row;    // or null
+    const int* end;            // offsets[experts]: rows in use
+    int pairs;
+};
+__device__ __forceinline__ long long row_looked_up(long long first, long long ctas) {   // by this thread, one of 256 from `first` on
+    return first + (long long)((threadIdx.x & 31) * (kRowThreads / 32) + (threadIdx.x >> 5)) * ctas;
+}
+__device__ __forceinline__ int pair_of(const RowTables& a, long long r) { return a.pair_of_row && r < a.pairs ? a.pair_of_row[r] : -1; }
+__device__ __forceinline__ int row_of(const RowTables& a, int p) { return p >= 0 && p < a.pairs ? a.row_of_pair[p] : -1; }
+// CTA `cta` of `ctas` sees to the rows cta, cta + ctas, ...: a lane looks one of its warp's up, the warp clears what its lanes
+// found.  `back` is row_of(pair_of()) of the thread's first row, asked for ahead of the CTA's work: two round trips at the end of
+// every CTA cost 1 us of a sort of 128 tokens x 8 and 6 us of 110 in the gradient of 2048 tokens x 8 x 6144.
+template <class Clear>
+__device__ __forceinline__ void clear_unnamed(const RowTables& a, long long cta, long long ctas, int back, Clear&& clear) {
+    const int end = min(max(*a.end, 0), a.pairs);
+    for (long long first = cta; first < a.pairs; first += ctas * kRowThreads) {
+        const long long r = row_looked_up(first, ctas);
+        if (first != cta) back = row_of(a, pair_of(a, r));
+        const bool named = !a.pair_of_row ? r < end : r < end ? back >= 0 && back < a.pairs : back == (int)r;
+        for (unsigned m = __ballot_sync(0xFFFFFFFFu, r < a.pairs && !named); m; m &= m - 1)
+            clear(first + (long long)((__ffs(m) - 1) * (kRowThreads / 32) + (int)(threadIdx.x >> 5)) * ctas);
+    }
 }
 
 // ---- sort: rows[row_of_pair[p]] = x[p / topk] -----------------------------------------------
@@ -283,7 +312,7 @@ struct SortArgs {
     const uint8_t* x_sf;       // scale bytes that travel with the rows, or null
     uint8_t* rows;
     uint8_t* rows_sf;
-    const int* end;            // offsets[experts]: rows in use
+    RowTables tables;
     long long x_stride, sf_stride;   // bytes between tokens
     int sf_bytes, sf_vec;
 };
@@ -318,9 +347,13 @@ __global__ void __launch_bounds__(kRowThreads) k_sort_rows(const SortArgs a) {
     const RowFrame& f = a.f;
     const RowCols<V, U> c(f);
     const long long steps = (f.tokens + (long long)gridDim.x * f.tall - 1) / ((long long)gridDim.x * f.tall);
+    const long long cta = (long long)blockIdx.y * gridDim.x + blockIdx.x, ctas = (long long)gridDim.x * gridDim.y;
     grid_wait();
+    const int pair = pair_of(a.tables, row_looked_up(cta, ctas));
+    int back = -1;
     for (long long step0 = 0; step0 < steps; step0 += f.batch) {
         row_fetch<false>(f, nullptr, 0, step0, s_row, nullptr);
+        if (step0 == 0) back = row_of(a.tables, pair);
         const int here = (int)min((long long)f.batch, steps - step0);
         for (int s = 0; s < here; ++s) {
             const long long t = ((step0 + s) * gridDim.x + blockIdx.x) * f.tall + c.row;
@@ -348,12 +381,10 @@ __global__ void __launch_bounds__(kRowThreads) k_sort_rows(const SortArgs a) {
             }
         }
     }
-    // rows behind the last expert's
-    const int end = min(max(*a.end, 0), f.pairs);
-    for (long long r = end + (long long)blockIdx.y * gridDim.x + blockIdx.x; r < f.pairs; r += (long long)gridDim.x * gridDim.y) {
+    clear_unnamed(a.tables, cta, ctas, back, [&](long long r) {
         clear_row<V>(a.rows + r * f.row_bytes, f.row_bytes);
         if (a.x_sf) clear_row<1>(a.rows_sf + r * a.sf_bytes, a.sf_bytes);
-    }
+    });
 }
 
 // ---- unsort: y[t] = sum_j w[t, j] rows[row_of_pair[t, j]] ------------------------------------
@@ -426,7 +457,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_unsort_rows(const UnsortArgs
 }
 
 // ---- gradient of the weighted unsort -----------------------------------------------------------
-// drows[row(t, j)] = w[t, j] dy[t];  dw[t, j] = <dy[t], rows[row(t, j)]>.  A team of 1, 2, 4 or 8 warps (by the row's
+// drows[row(t, j)] = w[t, j] dy[t], 0 in rows that no pair names;  dw[t, j] = <dy[t], rows[row(t, j)]>.  A team of 1, 2, 4 or 8 warps (by the row's
 // width) takes one token.  dy is read once per eight pairs, the eight rows' vectors are requested together; a dot is
 // summed per lane, over the warp, over the team, always in that order.
 // 2048 tokens x 8, 6144 bf16: 69 us = 6.2 TB/s; with the loads one after the other 92 us, and with the 64 registers that
@@ -437,11 +468,10 @@ struct UnsortGradArgs {
     const float* w;
     uint8_t* drows;            // or null
     float* dw;                 // [tokens][topk] or null
-    const int* row_of_pair;
-    const int* end;
+    RowTables tables;
     long long dy_stride, rows_stride, w_stride;
     int row_bytes;             // of drows (contiguous)
-    int tokens, topk, pairs, vecs, team;
+    int tokens, topk, vecs, team;
 };
 
 template <int kType, int V, bool kRows, bool kDots>
@@ -455,8 +485,13 @@ __global__ void __launch_bounds__(kRowThreads, 2) k_unsort_grad(const UnsortGrad
     const int teams = 8 / a.team, team = warp / a.team, member = warp - team * a.team;
     const int step = a.team * 32;
     const long long t = (long long)blockIdx.x * teams + team;
+    int pair = -1, back = -1;
+    if constexpr (kRows) {
+        pair = pair_of(a.tables, row_looked_up(blockIdx.x, gridDim.x));
+        if (t >= a.tokens) back = row_of(a.tables, pair);
+    }
     if (t < a.tokens) {
-        const int* rp = a.row_of_pair + t * a.topk;
+        const int* rp = a.tables.row_of_pair + t * a.topk;
         const uint8_t* dy = a.dy + t * a.dy_stride;
         for (int j0 = 0, turn = 0; j0 < a.topk; j0 += 8, turn ^= 1) {
             int r[8];
@@ -468,9 +503,10 @@ __global__ void __launch_bounds__(kRowThreads, 2) k_unsort_grad(const UnsortGrad
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if (r[j] >= a.pairs) r[j] = -1;
+                if (r[j] >= a.tables.pairs) r[j] = -1;
                 w[j] = r[j] >= 0 ? a.w[t * a.w_stride + j0 + j] : 0.0f;
             }
+            if (kRows && j0 == 0) back = row_of(a.tables, pair);
             for (int i = member * 32 + lane; i < a.vecs; i += step) {
                 const long long at = (long long)i * V;
                 const T g = *reinterpret_cast<const T*>(dy + at);
@@ -514,13 +550,12 @@ __global__ void __launch_bounds__(kRowThreads, 2) k_unsort_grad(const UnsortGrad
                     float sum = s_dot[turn][warp][lane];
                     for (int k = 1; k < a.team; ++k) sum += s_dot[turn][warp + k][lane];
                     const int own = rp[j0 + lane];
-                    a.dw[t * a.topk + j0 + lane] = own >= 0 && own < a.pairs ? sum : 0.0f;   // a dropped pair has no gradient, whatever dy holds
+                    a.dw[t * a.topk + j0 + lane] = own >= 0 && own < a.tables.pairs ? sum : 0.0f;   // a dropped pair has no gradient, whatever dy holds
                 }
             }
         }
     }
     if constexpr (kRows) {
-        const int end = min(max(*a.end, 0), a.pairs);
-        for (long long r = end + (long long)blockIdx.x; r < a.pairs; r += gridDim.x) clear_row<V>(a.drows + r * a.row_bytes, a.row_bytes);
+        clear_unnamed(a.tables, blockIdx.x, gridDim.x, back, [&](long long r) { clear_row<V>(a.drows + r * a.row_bytes, a.row_bytes); });
     }
 }

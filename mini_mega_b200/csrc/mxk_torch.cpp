@@ -138,7 +138,7 @@ void check_leaf_under_capture(const char* fn, const Tensor& t) {
                                  "another stream; drop its outputs before the capture begins");
 }
 
-Tensor sort_rows(const Tensor& x_in, const Tensor& row_of_pair, const Tensor& offsets, const Tensor& sf_in, Tensor* rows_sf) {
+Tensor sort_rows(const Tensor& x_in, const Tensor& row_of_pair, const Tensor& pair_of_row, const Tensor& offsets, const Tensor& sf_in, Tensor* rows_sf) {
     const c10::cuda::CUDAGuard guard(x_in.device());
     const int64_t tokens = row_of_pair.size(0), topk = row_of_pair.size(1);
     const Tensor x = rows_contiguous(x_in);
@@ -147,11 +147,11 @@ Tensor sort_rows(const Tensor& x_in, const Tensor& row_of_pair, const Tensor& of
         sf = rows_contiguous(sf_in);
         *rows_sf = fresh({tokens * topk, sf.size(1)}, at::kByte, sf);
     }
-    done(mxk_sort_tokens(x.data_ptr(), row_bytes_apart(x), x.size(1) * (int64_t)x.element_size(), sf.defined() ? sf.data_ptr() : nullptr,
-                         sf.defined() ? sf.stride(0) : 0, sf.defined() ? sf.size(1) : 0, (int32_t)tokens, (int32_t)topk,
-                         (int32_t)(offsets.size(0) - 1), table(row_of_pair), table(offsets), rows.data_ptr(),
-                         sf.defined() ? rows_sf->data_ptr() : nullptr, stream_of(x)),
-         "mxk_sort_tokens");
+    done(mxk_sort_tokens_by_plan(x.data_ptr(), row_bytes_apart(x), x.size(1) * (int64_t)x.element_size(), sf.defined() ? sf.data_ptr() : nullptr,
+                                 sf.defined() ? sf.stride(0) : 0, sf.defined() ? sf.size(1) : 0, (int32_t)tokens, (int32_t)topk,
+                                 (int32_t)(offsets.size(0) - 1), table(row_of_pair), table(pair_of_row), table(offsets), rows.data_ptr(),
+                                 sf.defined() ? rows_sf->data_ptr() : nullptr, stream_of(x)),
+         "mxk_sort_tokens_by_plan");
     return rows;
 }
 
@@ -170,43 +170,43 @@ Tensor unsort_rows(const Tensor& rows_in, const Tensor& weights_in, const Tensor
 
 // Sort and plain unsort are linear and each other's gradient, so they can be differentiated again;
 // the weighted unsort cannot, and says so.
-Tensor sort_differentiable(const Tensor& x, const Tensor& row_of_pair, const Tensor& offsets);
-Tensor unsort_differentiable(const Tensor& rows, const Tensor& weights, const Tensor& row_of_pair, const Tensor& offsets);
+Tensor sort_differentiable(const Tensor& x, const Tensor& row_of_pair, const Tensor& pair_of_row, const Tensor& offsets);
+Tensor unsort_differentiable(const Tensor& rows, const Tensor& weights, const Tensor& row_of_pair, const Tensor& pair_of_row, const Tensor& offsets);
 
 struct SortFunction : torch::autograd::Function<SortFunction> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& row_of_pair, const Tensor& offsets) {
-        ctx->save_for_backward({row_of_pair, offsets});
-        return sort_rows(x, row_of_pair, offsets, Tensor(), nullptr);
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& row_of_pair, const Tensor& pair_of_row, const Tensor& offsets) {
+        ctx->save_for_backward({row_of_pair, pair_of_row, offsets});
+        return sort_rows(x, row_of_pair, pair_of_row, offsets, Tensor(), nullptr);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         not_followed("sort_tokens_by_expert (backward)", {&grads[0]});
-        return {unsort_differentiable(grads[0], Tensor(), saved[0], saved[1]), Tensor(), Tensor()};
+        return {unsort_differentiable(grads[0], Tensor(), saved[0], saved[1], saved[2]), Tensor(), Tensor(), Tensor()};
     }
 };
 
 struct SumFunction : torch::autograd::Function<SumFunction> {   // unsort without weights
-    static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& row_of_pair, const Tensor& offsets) {
-        ctx->save_for_backward({row_of_pair, offsets});
+    static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& row_of_pair, const Tensor& pair_of_row, const Tensor& offsets) {
+        ctx->save_for_backward({row_of_pair, pair_of_row, offsets});
         return unsort_rows(rows, Tensor(), row_of_pair);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         not_followed("unsort_tokens_by_expert (backward)", {&grads[0]});
-        return {sort_differentiable(grads[0], saved[0], saved[1]), Tensor(), Tensor()};
+        return {sort_differentiable(grads[0], saved[0], saved[1], saved[2]), Tensor(), Tensor(), Tensor()};
     }
 };
 
 struct UnsortFunction : torch::autograd::Function<UnsortFunction> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& weights, const Tensor& row_of_pair, const Tensor& offsets) {
+    static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& weights, const Tensor& row_of_pair, const Tensor& pair_of_row, const Tensor& offsets) {
         // rows are kept for the gradient of the weights only
-        ctx->save_for_backward({weights.requires_grad() ? rows : Tensor(), weights, row_of_pair, offsets});
+        ctx->save_for_backward({weights.requires_grad() ? rows : Tensor(), weights, row_of_pair, pair_of_row, offsets});
         ctx->saved_data["rows_grad"] = rows.requires_grad();
         return unsort_rows(rows, weights, row_of_pair);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &weights_in = saved[1], &row_of_pair = saved[2], &offsets = saved[3];
+        const Tensor &weights_in = saved[1], &row_of_pair = saved[2], &pair_of_row = saved[3], &offsets = saved[4];
         not_followed("unsort_tokens_by_expert (backward)", {&grads[0]});
         if (at::GradMode::is_enabled()) throw std::runtime_error("unsort_tokens_by_expert: the weighted sum has no second derivative (create_graph)");
         const c10::cuda::CUDAGuard guard(grads[0].device());
@@ -216,25 +216,25 @@ struct UnsortFunction : torch::autograd::Function<UnsortFunction> {
         Tensor drows, dweights;
         if (ctx->saved_data["rows_grad"].toBool()) drows = fresh({tokens * topk, dy.size(1)}, dy.scalar_type(), dy);
         if (rows.defined()) dweights = fresh({tokens, topk}, at::kFloat, weights);
-        done(mxk_unsort_tokens_grad(dy.data_ptr(), row_bytes_apart(dy), rows.defined() ? rows.data_ptr() : nullptr,
+        done(mxk_unsort_tokens_grad_by_plan(dy.data_ptr(), row_bytes_apart(dy), rows.defined() ? rows.data_ptr() : nullptr,
                                     rows.defined() ? row_bytes_apart(rows) : 0, type_code(dy.scalar_type()),
                                     static_cast<const float*>(weights.data_ptr()), weights.stride(0), (int32_t)tokens, (int32_t)topk,
-                                    (int32_t)(offsets.size(0) - 1), (int32_t)dy.size(1), table(row_of_pair), table(offsets),
+                                    (int32_t)(offsets.size(0) - 1), (int32_t)dy.size(1), table(row_of_pair), table(pair_of_row), table(offsets),
                                     drows.defined() ? drows.data_ptr() : nullptr,
                                     dweights.defined() ? static_cast<float*>(dweights.data_ptr()) : nullptr, stream_of(dy)),
-             "mxk_unsort_tokens_grad");
-        return {drows, dweights, Tensor(), Tensor()};
+             "mxk_unsort_tokens_grad_by_plan");
+        return {drows, dweights, Tensor(), Tensor(), Tensor()};
     }
 };
 
-Tensor sort_differentiable(const Tensor& x, const Tensor& row_of_pair, const Tensor& offsets) {
-    if (!at::GradMode::is_enabled() || !x.requires_grad()) return sort_rows(x, row_of_pair, offsets, Tensor(), nullptr);
-    return SortFunction::apply(x, row_of_pair, offsets);
+Tensor sort_differentiable(const Tensor& x, const Tensor& row_of_pair, const Tensor& pair_of_row, const Tensor& offsets) {
+    if (!at::GradMode::is_enabled() || !x.requires_grad()) return sort_rows(x, row_of_pair, pair_of_row, offsets, Tensor(), nullptr);
+    return SortFunction::apply(x, row_of_pair, pair_of_row, offsets);
 }
-Tensor unsort_differentiable(const Tensor& rows, const Tensor& weights, const Tensor& row_of_pair, const Tensor& offsets) {
+Tensor unsort_differentiable(const Tensor& rows, const Tensor& weights, const Tensor& row_of_pair, const Tensor& pair_of_row, const Tensor& offsets) {
     if (!at::GradMode::is_enabled() || !(rows.requires_grad() || (weights.defined() && weights.requires_grad())))
         return unsort_rows(rows, weights, row_of_pair);
-    return weights.defined() ? UnsortFunction::apply(rows, weights, row_of_pair, offsets) : SumFunction::apply(rows, row_of_pair, offsets);
+    return weights.defined() ? UnsortFunction::apply(rows, weights, row_of_pair, pair_of_row, offsets) : SumFunction::apply(rows, row_of_pair, pair_of_row, offsets);
 }
 
 bool byte_type(at::ScalarType t) { return t == at::kFloat8_e4m3fn || t == at::kFloat8_e5m2 || t == at::kByte || t == at::kChar; }
@@ -255,12 +255,12 @@ py::object sort_tokens(const Tensor& x, const Tensor& row_of_pair, const Tensor&
     MXK_TYPE(!grad || type_code(x.scalar_type()) >= 0, fn, ": only bf16, fp16 and fp32 rows have a gradient");
     if (x_sf) {
         Tensor rows_sf;
-        const Tensor rows = sort_rows(x, row_of_pair, offsets, *x_sf, &rows_sf);
+        const Tensor rows = sort_rows(x, row_of_pair, pair_of_row, offsets, *x_sf, &rows_sf);
         return py::cast(std::make_pair(rows, rows_sf));
     }
     const c10::cuda::CUDAGuard guard(x.device());
     if (grad && under_capture()) check_leaf_under_capture(fn, x);
-    return py::cast(sort_differentiable(x, row_of_pair, offsets));
+    return py::cast(sort_differentiable(x, row_of_pair, pair_of_row, offsets));
 }
 
 Tensor unsort_tokens(const Tensor& rows, const Tensor& row_of_pair, const Tensor& pair_of_row, const Tensor& offsets, const MaybeTensor& topk_weights) {
@@ -280,7 +280,7 @@ Tensor unsort_tokens(const Tensor& rows, const Tensor& row_of_pair, const Tensor
         check_leaf_under_capture(fn, rows);
         check_leaf_under_capture(fn, weights);
     }
-    return unsort_differentiable(rows, weights, row_of_pair, offsets);
+    return unsort_differentiable(rows, weights, row_of_pair, pair_of_row, offsets);
 }
 
 // ---- 8-bit products -----------------------------------------------------------------------

@@ -29,8 +29,10 @@ class ExpertPlan(NamedTuple):
     ``pair_of_row`` ``[tokens * topk]``: its inverse, -1 behind the last row in use.
     ``offsets`` ``[num_experts + 1]``: expert e's rows are ``offsets[e] .. offsets[e + 1]``.
 
-    ``plan_tokens_by_expert`` builds it; tables of one's own in the same form serve as well (an entry out of
-    range counts as a dropped pair; two pairs with one row are the caller's mistake)."""
+    ``plan_tokens_by_expert`` builds it; tables of one's own in the same form serve as well.  An entry of
+    ``row_of_pair`` out of range counts as a dropped pair, also one that had a row when the plan was made: that row, which no
+    pair names any more, is zero in sorted rows and in gradients.  (Two pairs with one row, or a ``pair_of_row`` that is not the
+    inverse of what is kept, are the caller's mistake.)"""
     row_of_pair: torch.Tensor
     pair_of_row: torch.Tensor
     offsets: torch.Tensor
@@ -45,7 +47,8 @@ def plan_tokens_by_expert(topk_idx: torch.Tensor, num_experts: int, first_expert
 
 def sort_tokens_by_expert(x: torch.Tensor, plan: ExpertPlan, x_sf: Optional[torch.Tensor] = None):
     """The rows of ``x`` ``[tokens, hidden]`` in expert order, ``[tokens * topk, hidden]``: row
-    ``plan.row_of_pair[t, j]`` is ``x[t]``.  Rows behind ``plan.offsets[-1]`` (as many as pairs were dropped) are zero.
+    ``plan.row_of_pair[t, j]`` is ``x[t]``.  Rows that no pair names (those behind ``plan.offsets[-1]``, as many as pairs were
+    dropped) are zero.
 
     ``x`` is bf16, fp16 or fp32 (differentiable: the gradient of a token is the sum over its rows, in FP32), or 8-bit;
     with ``x_sf`` (uint8 ``[tokens, ...]`` scale bytes) the scales travel along and ``(rows, rows_sf)`` is returned."""
@@ -57,6 +60,6 @@ def unsort_tokens_by_expert(rows: torch.Tensor, plan: ExpertPlan, topk_weights: 
     rows[plan.row_of_pair[t, j]]`` (j ascending, in FP32, rounded once), dropped pairs left out; without weights the
     plain sum.  ``rows`` ``[tokens * topk, hidden]`` is bf16, fp16 or fp32, ``topk_weights`` fp32 ``[tokens, topk]``.
 
-    Differentiable in ``rows`` (rows behind ``plan.offsets[-1]`` get zeros) and in ``topk_weights`` (dropped pairs get 0);
+    Differentiable in ``rows`` (rows that no pair names get zeros) and in ``topk_weights`` (dropped pairs get 0);
     a second time only without weights."""
     return _lib.ops().unsort_tokens(rows, *plan, topk_weights)

@@ -132,3 +132,63 @@ def test_scales_of_very_wide_rows(blocks):
         at = order[first:min(first + 100, end)]
         assert torch.equal(rows[first:first + len(at)], x[at]) and torch.equal(rows_sf[first:first + len(at)], sf[at])
     assert not rows[end:].any() and not rows_sf[end:].any()
+
+
+# ---------------------------------------------------------- pairs dropped from the tables after the plan was made
+def _over_capacity(tokens, topk, experts, capacity, both_tables):
+    """A plan whose pairs beyond `capacity` of an expert are then dropped: (the tables, the pair of every row or -1)."""
+    g = torch.Generator(device="cuda").manual_seed(tokens + topk)
+    idx = torch.randint(-1, experts, (tokens, topk), device="cuda", generator=g)
+    plan = mm.plan_tokens_by_expert(idx, experts)
+    place = torch.arange(tokens * topk, device="cuda")
+    owner = torch.searchsorted(plan.offsets[1:].contiguous(), place.int(), right=True).clamp(max=experts - 1)
+    left = (plan.pair_of_row >= 0) & (place - plan.offsets[owner] < capacity)
+    row = plan.row_of_pair
+    dropped = (row >= 0) & ~left[row.clamp(min=0).long()]
+    named = torch.where(left, plan.pair_of_row, -1)
+    return plan._replace(row_of_pair=torch.where(dropped, -1, row), pair_of_row=named if both_tables else plan.pair_of_row), named.long()
+
+
+def _soil(shape, dtype):
+    """Leaves the allocator with a freed block of this size that holds NaN."""
+    torch.full(shape, float("nan"), device="cuda").to(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("both_tables", [False, True])
+@pytest.mark.parametrize("tokens, topk, experts, capacity, hidden, dtype", [
+    (40, 4, 5, 20, 64, torch.bfloat16), (300, 8, 16, 100, 127, torch.float16), (1000, 6, 60, 70, 1001, torch.float32),
+    (1, 8, 2, 2, 6144, torch.bfloat16), (1, 8, 2, 1, 6144, torch.bfloat16), (4096, 256, 3, 200000, 3, torch.float16)])
+def test_rows_of_pairs_dropped_after_the_plan_are_zero(tokens, topk, experts, capacity, hidden, dtype, both_tables):
+    """In the sorted rows and in every gradient of rows: whatever stands there takes part in the experts' products and in
+    the gradients of their weights."""
+    plan, named = _over_capacity(tokens, topk, experts, capacity, both_tables)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    rnd = lambda *s: torch.randn(s, device="cuda", generator=g)   # noqa: E731
+    x, w = rnd(tokens, hidden).to(dtype), rnd(tokens, topk)
+    at, held = named.clamp(min=0), (named >= 0)[:, None]
+    spread = torch.where(held, x[at // topk], torch.zeros((), dtype=dtype, device="cuda"))
+    _soil((tokens * topk, hidden), dtype)
+    assert torch.equal(mm.sort_tokens_by_expert(x, plan), spread)
+    rows, weights = rnd(tokens * topk, hidden).to(dtype).requires_grad_(), w.requires_grad_()
+    want = torch.where(held, (w.detach().view(-1)[at][:, None] * x[at // topk].float()).to(dtype), torch.zeros((), dtype=dtype, device="cuda"))
+    y = mm.unsort_tokens_by_expert(rows, plan, weights)
+    _soil((tokens * topk, hidden), dtype)
+    drows, dw = torch.autograd.grad(y, (rows, weights), x)
+    assert torch.equal(drows, want) and bool((dw[plan.row_of_pair < 0] == 0).all())   # one FP32 product, rounded once
+    y = mm.unsort_tokens_by_expert(rows, plan)
+    _soil((tokens * topk, hidden), dtype)
+    assert torch.equal(torch.autograd.grad(y, rows, x)[0], spread)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("both_tables", [False, True])
+@pytest.mark.parametrize("blocks", [1, 7, 48])
+def test_scales_of_pairs_dropped_after_the_plan_are_zero(blocks, both_tables):
+    plan, named = _over_capacity(100, 4, 6, 50, both_tables)
+    x = torch.randint(1, 100, (100, 128 * blocks), device="cuda", dtype=torch.uint8)
+    sf = torch.randint(1, 100, (100, blocks), device="cuda", dtype=torch.uint8)
+    torch.full((400, 128 * blocks), 255, device="cuda", dtype=torch.uint8), torch.full((400, blocks), 255, device="cuda", dtype=torch.uint8)
+    rows, rows_sf = mm.sort_tokens_by_expert(x, plan, sf)
+    held = (named >= 0)[:, None]
+    assert torch.equal(rows, torch.where(held, x[named.clamp(min=0) // 4], 0)) and torch.equal(rows_sf, torch.where(held, sf[named.clamp(min=0) // 4], 0))
