@@ -447,6 +447,10 @@ typedef struct MxkMatmulArgs {
                                 * product is healthy would leave with its copies and MMAs under way    */
 } MxkMatmulArgs;
 int mxk_fp8_matmul(const MxkMatmulArgs* a, void* stream);
+/* How mxk_fp8_matmul cuts a product of these sizes (grouped: nonzero for a product with offsets); host only, needs no
+ * device.  cut[0]: 1 for pairs of CTAs with 256 weight rows per tile, 0 for single ones with 128; cut[1]: rows of x per tile at most;
+ * cut[2]: CTAs that share a tile's depth. */
+int mxk_matmul_cut(int32_t rows, int32_t cols, int32_t depth, int32_t experts, int32_t grouped, int32_t cut[3]);
 /* Synchronous: 0, or the MXK_DEV_* code of the first product on this device whose wait expired (its output is
  * then undefined). */
 int mxk_matmul_status(int32_t* out);

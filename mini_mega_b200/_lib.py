@@ -126,7 +126,7 @@ EXPORTS = [
     "mxk_read_status_static", "mxk_rwk_ticks_off", "mxk_ticks_count", "mxk_set_ticks", "mxk_select_win",
     "mxk_group_ranks", "mxk_gs_schedule_member", "mxk_gs_schedule_member_hot", "mxk_gs_group_skewed", "mxk_lpt_assign", "mxk_gs_schedule_on_device",
     "mxk_plan_tokens", "mxk_sort_tokens", "mxk_sort_tokens_by_plan", "mxk_unsort_tokens", "mxk_unsort_tokens_grad", "mxk_unsort_tokens_grad_by_plan",
-    "mxk_fp8_matmul", "mxk_matmul_status",
+    "mxk_fp8_matmul", "mxk_matmul_cut", "mxk_matmul_status",
     "mxk_symm_alloc", "mxk_symm_free", "mxk_ipc_export", "mxk_ipc_import", "mxk_ipc_close",
 ]
 
@@ -183,6 +183,7 @@ def lib():
     L.mxk_unsort_tokens_grad.argtypes = [vp, i64, vp, i64, i32, vp, i64, i32, i32, i32, i32, vp, vp, vp, vp, vp]
     L.mxk_unsort_tokens_grad_by_plan.argtypes = [vp, i64, vp, i64, i32, vp, i64, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp]
     L.mxk_fp8_matmul.argtypes = [C.POINTER(MxkMatmulArgs), vp]
+    L.mxk_matmul_cut.argtypes = [i32, i32, i32, i32, i32, C.POINTER(C.c_int32)]
     L.mxk_matmul_status.argtypes = [C.POINTER(C.c_int32)]
     L.mxk_symm_alloc.argtypes = [C.POINTER(C.c_void_p), C.c_int64]
     L.mxk_symm_free.argtypes = [C.c_void_p]

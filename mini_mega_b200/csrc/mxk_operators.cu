@@ -186,14 +186,15 @@ int unroll_of(int vec) { return vec >= 16 ? 1 : vec == 8 ? 2 : 4; }
 //                                     0.6 ns x rows (128 rows: 230, 192: 267, 224: 279)
 //   a further round of tiles          0.25
 //   partial sums between splits       0.8 + full (1.1 + 0.018 x rows)
-// and, beside them, the operands' way from memory (6.3 TB/s) and, for every tile of rows after a group's first, its
-// weights' way from L2 once more (12 TB/s).  Both sides, measured: 1 x 4096 x 6144 in 1 / 2 / 4 splits 11.3 / 8.7 /
-// 8.0 us; 16 x 1024 x 2048 6.3 / 6.5 / 5.5; 128 x 4096 x 7168 tiles of 64 rows in 2 splits 12.2, of 32 rows unsplit 13.6;
-// 512 x 4096 x 7168 single 17.5, pairs 20.1; 2048 x 4096 x 7168 single 57, pairs 52; 32 groups of 200 rows x 4096 x 7168
-// pairs with one tile a group 192, with two 282, single CTAs with two 252.  Splits only while every tile runs at once: a
-// second round costs 7 us (20 groups of 40 rows x 1000 x 2992: 21 us without splits, 24 in two, 45 in four), and 8 of them
-// only for a few tiles, because few clusters of eight fit the GPU at once (1 x 2048 x 6144: 14.3 us, in four 8.8).
-// Of 55 products, dense and grouped, 53 ran within 5 % of the best of all cuts, the others within 11 %.
+// and, for grouped products only, the operands' way from memory (6.3 TB/s; dense ones are bound by it in no cut that the parts
+// above do not tell apart already) and, for every tile of rows after a group's first, its weights' way from L2 once more
+// (12 TB/s).  Both sides, measured: 1 x 4096 x 6144 in 1 / 2 / 4 splits 11.3 / 8.7 / 8.0 us; 16 x 1024 x 2048 6.3 / 6.5 / 5.5;
+// 128 x 4096 x 7168 tiles of 64 rows in 2 splits 12.2, of 32 rows unsplit 13.6; 512 x 4096 x 7168 single 17.5, pairs 20.1;
+// 2048 x 4096 x 7168 single 57, pairs 52; 32 groups of 200 rows x 4096 x 7168 pairs with one tile a group 192, with two 282,
+// single CTAs with two 252.  Splits only while every tile is expected to run at once (unevenly loaded groups can have more
+// tiles than their mean tells: some clusters then take a second one): a second round costs 7 us (20 groups of 40 rows x
+// 1000 x 2992: 21 us without splits, 24 in two, 45 in four), and 8 of them only for a few tiles, because few clusters of
+// eight fit the GPU at once (1 x 2048 x 6144: 14.3 us, in four 8.8).
 struct MmShape { bool pair; int bt, splits; };
 MmShape mm_shape(int64_t rows, int64_t cols, int64_t depth, int64_t experts, bool grouped) {
     const int nkb = (int)((depth + 127) / 128), k_groups = (nkb + 3) / 4;
@@ -233,6 +234,10 @@ MmShape mm_shape(int64_t rows, int64_t cols, int64_t depth, int64_t experts, boo
 // (grid_wait in every role), and the longest wait (a tile's whole K loop) gets 4 us per
 // K block on top, more than ten times what one takes.
 constexpr int kMmLeastSpins = 8000000;
+
+bool bad_product(int64_t rows, int64_t cols, int64_t depth, int64_t experts) {
+    return rows < 0 || cols < 1 || depth < 16 || depth % 16 || rows > (1 << 30) || depth > (1 << 30) || experts < 1 || experts > kMmMaxExperts || experts * cols > (1 << 30);
+}
 
 int dtype_bytes(int dtype) { return dtype == MXK_DTYPE_FP32 ? 4 : 2; }
 
@@ -373,7 +378,7 @@ int mxk_unsort_tokens_grad_by_plan(const void* dy, int64_t dy_stride, const void
 int mxk_fp8_matmul(const MxkMatmulArgs* p, void* stream) {
     if (!p) return fail(MXK_ERR_BAD_ARG, "fp8_matmul: null arguments");
     const int64_t rows = p->rows, cols = p->cols, depth = p->depth, experts = p->offsets ? p->experts : 1;
-    if (rows < 0 || cols < 1 || depth < 16 || depth % 16 || rows > (1 << 30) || depth > (1 << 30) || experts < 1 || experts > kMmMaxExperts || experts * cols > (1 << 30))
+    if (bad_product(rows, cols, depth, experts))
         return fail(MXK_ERR_BAD_ARG, "fp8_matmul: need depth a multiple of 16, 1 <= experts <= 1024, rows and experts * cols <= 2^30");
     if (p->x_format < MXK_FP8_E4M3 || p->x_format > MXK_FP8_E5M2 || p->w_format < MXK_FP8_E4M3 || p->w_format > MXK_FP8_E5M2)
         return fail(MXK_ERR_BAD_ARG, "fp8_matmul: operand formats are MXK_FP8_E4M3 and MXK_FP8_E5M2");
@@ -422,6 +427,13 @@ int mxk_fp8_matmul(const MxkMatmulArgs* p, void* stream) {
     if (tiles_most > (1 << 30)) return fail(MXK_ERR_BAD_ARG, "fp8_matmul: more than 2^30 tiles");
     const dim3 grid((unsigned)(std::min<int64_t>(tiles_most, kSms / cluster) * cluster), 1, 1);
     return launched(launch(fn, grid, kMmThreads, (size_t)smem, cluster, static_cast<cudaStream_t>(stream), a, tm_x, tm_w), "launch k_matmul");
+}
+
+int mxk_matmul_cut(int32_t rows, int32_t cols, int32_t depth, int32_t experts, int32_t grouped, int32_t cut[3]) {
+    if (!cut || rows < 1 || bad_product(rows, cols, depth, grouped ? experts : 1)) return fail(MXK_ERR_BAD_ARG, "matmul_cut: null argument or sizes out of range");
+    const MmShape sh = mm_shape(rows, cols, depth, grouped ? experts : 1, grouped != 0);
+    cut[0] = sh.pair; cut[1] = sh.bt; cut[2] = sh.splits;
+    return 0;
 }
 
 int mxk_matmul_status(int32_t* out) {
