@@ -186,9 +186,8 @@ int unroll_of(int vec) { return vec >= 16 ? 1 : vec == 8 ? 2 : 4; }
 //                                     0.6 ns x rows (128 rows: 230, 192: 267, 224: 279)
 //   a further round of tiles          0.25
 //   partial sums between splits       0.8 + full (1.1 + 0.018 x rows)
-// and, for grouped products only, the operands' way from memory (6.3 TB/s; dense ones are bound by it in no cut that the parts
-// above do not tell apart already) and, for every tile of rows after a group's first, its weights' way from L2 once more
-// (12 TB/s).  Both sides, measured: 1 x 4096 x 6144 in 1 / 2 / 4 splits 11.3 / 8.7 / 8.0 us; 16 x 1024 x 2048 6.3 / 6.5 / 5.5;
+// and, for grouped products only, the operands' way from memory (6.3 TB/s) and, for every tile of rows after a group's first,
+// its weights' way from L2 once more (12 TB/s).  Both sides, measured: 1 x 4096 x 6144 in 1 / 2 / 4 splits 11.3 / 8.7 / 8.0 us; 16 x 1024 x 2048 6.3 / 6.5 / 5.5;
 // 128 x 4096 x 7168 tiles of 64 rows in 2 splits 12.2, of 32 rows unsplit 13.6; 512 x 4096 x 7168 single 17.5, pairs 20.1;
 // 2048 x 4096 x 7168 single 57, pairs 52; 32 groups of 200 rows x 4096 x 7168 pairs with one tile a group 192, with two 282,
 // single CTAs with two 252.  Splits only while every tile is expected to run at once (unevenly loaded groups can have more

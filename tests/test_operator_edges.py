@@ -192,3 +192,49 @@ def test_scales_of_pairs_dropped_after_the_plan_are_zero(blocks, both_tables):
     rows, rows_sf = mm.sort_tokens_by_expert(x, plan, sf)
     held = (named >= 0)[:, None]
     assert torch.equal(rows, torch.where(held, x[named.clamp(min=0) // 4], 0)) and torch.equal(rows_sf, torch.where(held, sf[named.clamp(min=0) // 4], 0))
+
+
+# ------------------------------------------------------------------- a training step whose bound holds by construction
+@pytest.mark.gpu
+def test_training_step_with_the_routing_held():
+    """Sort, two products with a relu between them, unsort, and all gradients, FP32 against 64 bits.  Routing and weights are
+    inputs, the same ones in every run, so the run on magnitudes adds up the magnitude of every term that the signed run adds (relu
+    passes all of them, at least what it passes there): a result that is a chain of n roundings of 2^-24 is off by at most
+    n 2^-24 (1 + n 2^-24) of it, element for element.  n: both depths, topk, the rows (gradients of the experts' weights), one
+    product each.  No relu may change its side: the values there are farther from zero than their own bound."""
+    tokens, topk, experts, hidden, inter = 50, 3, 5, 24, 32
+    g = torch.Generator().manual_seed(8)
+    rnd = lambda *s: torch.randn(*s, generator=g)   # noqa: E731
+    x, w1, w2, dy = rnd(tokens, hidden), rnd(experts, inter, hidden), rnd(experts, hidden, inter), rnd(tokens, hidden)
+    weights, idx = torch.softmax(rnd(tokens, topk), 1), torch.randint(-1, experts, (tokens, topk), generator=g)
+    idx[5] = -1
+    flat = idx.view(-1)
+    order = torch.sort(torch.where(flat < 0, experts, flat), stable=True).indices
+    offsets = [0] + torch.tensor([int((flat == e).sum()) for e in range(experts)]).cumsum(0).tolist()
+    inner = []
+
+    def step(x, weights, w1, w2, dy, sort, unsort):
+        rows = sort(x)
+        parts = [rows[a:b] @ w1[e].t() for e, (a, b) in enumerate(zip(offsets, offsets[1:]))]
+        inner.append(torch.cat(parts).detach().double().cpu())
+        out = torch.cat([p.relu() @ w2[e].t() for e, p in enumerate(parts)] + [rows.new_zeros(rows.shape[0] - offsets[-1], hidden)])
+        y = unsort(out, weights)
+        return (y.detach(), *torch.autograd.grad(y, (x, weights, w1, w2), dy))
+
+    def plain_unsort(out, weights):
+        n = offsets[-1]
+        parts = out[:n] * weights.reshape(-1)[order[:n], None]
+        return torch.zeros(tokens, hidden, dtype=out.dtype).index_add(0, order[:n] // topk, parts)
+
+    plan = mm.plan_tokens_by_expert(idx.cuda(), experts)
+    assert plan.offsets.tolist() == offsets
+    leaves = (x, weights, w1, w2)
+    plain = lambda f, d: step(*[f(t.double()).requires_grad_() for t in leaves], d, lambda t: t[order // topk], plain_unsort)   # noqa: E731
+    want, mass = plain(lambda t: t, dy.double()), plain(torch.abs, dy.double().abs())
+    got = step(*[t.cuda().requires_grad_() for t in leaves], dy.cuda(), lambda t: mm.sort_tokens_by_expert(t, plan),
+               lambda out, w: mm.unsort_tokens_by_expert(out, plan, w))
+    assert bool((inner[0].abs() > hidden * 2.0 ** -23 * inner[1]).all())
+    n = hidden + inter + topk + offsets[-1] + 5
+    for name, a, b, m in zip(("y", "x", "weights", "w1", "w2"), got, want, mass):
+        tol = n * 2.0 ** -24 * (1 + n * 2.0 ** -24) * m
+        assert bool(((a.double().cpu() - b).abs() <= tol).all()), name
