@@ -313,7 +313,7 @@ Tensor matmul(const char* fn, const Tensor& x, const MaybeTensor& x_sf, const Te
     }
     const auto misaligned = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) & 15; };
     MXK_VALUE(x.stride(1) == 1 && (rows <= 1 || (x.stride(0) >= depth && x.stride(0) % 16 == 0)) && !misaligned(x), fn, ": x needs contiguous rows, 16-byte aligned and not overlapping");
-    const int64_t w_stride = cols > 1 ? w.stride(-2) : depth;
+    const int64_t w_stride = cols > 1 ? w.stride(-2) : experts > 1 ? w.stride(0) : depth;
     MXK_VALUE(w.stride(-1) == 1 && w_stride >= depth && w_stride % 16 == 0 && !misaligned(w) && (experts == 1 || w.stride(0) == cols * w_stride), fn, ": w needs contiguous rows, 16-byte aligned, and the experts' matrices one behind the other");
     if (offsets) {
         MXK_VALUE(offsets->scalar_type() == at::kInt && offsets->dim() == 1 && offsets->size(0) == experts + 1 && offsets->is_contiguous(), fn, ": offsets must be a contiguous int32 tensor of ", experts + 1, " entries");

@@ -238,3 +238,23 @@ def test_training_step_with_the_routing_held():
     for name, a, b, m in zip(("y", "x", "weights", "w1", "w2"), got, want, mass):
         tol = n * 2.0 ** -24 * (1 + n * 2.0 ** -24) * m
         assert bool(((a.double().cpu() - b).abs() <= tol).all()), name
+
+
+# ------------------------------------------------------------------------------- weights of one row, apart
+def test_experts_of_one_row_may_be_apart():
+    w, off = torch.zeros((3, 1, 160), dtype=E4)[..., :128], torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):     # of its layout there is nothing to say
+        mm.fp8_grouped_matmul(torch.zeros((4, 128), dtype=E4), w, off)
+    for bad in (torch.zeros((1, 1, 128), dtype=E4).expand(3, 1, 128), torch.zeros((3, 1, 136), dtype=E4)[..., :128]):
+        with pytest.raises(ValueError, match="w needs"):
+            mm.fp8_grouped_matmul(torch.zeros((4, 128), dtype=E4), bad, off)
+
+
+@pytest.mark.gpu
+def test_experts_of_one_row_apart():
+    g = torch.Generator(device="cuda").manual_seed(1)
+    small = lambda *s: torch.randint(-3, 4, s, device="cuda", generator=g).float().to(E4)   # noqa: E731
+    x, w = small(50, 272), small(4, 3, 304)[:, 1:2, 16:288]
+    off = torch.tensor([0, 20, 20, 45, 50], dtype=torch.int32, device="cuda")
+    want = torch.cat([x[a:b].double() @ w[e].double().t() for e, (a, b) in enumerate(zip(off.tolist(), off.tolist()[1:]))])
+    assert torch.equal(mm.fp8_grouped_matmul(x, w, off), want.to(torch.bfloat16))
