@@ -45,7 +45,7 @@ constexpr int kMmFirstEpi = 4;
 constexpr int kMmMaxStages = 8;
 constexpr int kMmMaxSfSlots = 8;
 constexpr int kMmSfTile = 512;                 // 128 rows x 4 scale bytes
-constexpr int kMmStageKb = 2, kMmPairStageKb = 2;   // K blocks of a ring stage
+constexpr int kMmStageKb = 2;                  // K blocks of a ring stage
 constexpr int kMmRowsMax = 224;                // columns of an accumulator: 2 x 224 leave 64 TMEM columns to the scales
 constexpr int kMmWBytes = 128 * 128;           // weight tile of one K block
 constexpr int kMmMaxExperts = 1024;
@@ -62,7 +62,7 @@ struct MmArgs {
     int n_tiles;               // weight tiles of a group
     int bt_max, box;           // rows of x per tile at most; rows per TMA box (pairs: half of them)
     int n_stages, sf_slots, sf_col;
-    int splits;                // CTAs (pairs) of a cluster that share a tile's K extent: 1, 2, 4 or 8
+    int splits;                // CTAs of a cluster that share a tile's K extent: 1, 2, 4 or 8; pairs take it whole
     int w_sf_rows, w_per_row;  // rows of a group's weight scale plane; 1: one scale row per weight row
     int zero_tail;             // clear out rows behind the last group
     FastDiv fbt, fnt;          // division by bt_max and n_tiles
@@ -154,36 +154,37 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
     return p != 0;
 }
-// commit of a pair's MMAs onto the barrier at this offset in both CTAs of the pair that starts at
-// cluster rank `first` (a signal inside one cluster; no load, no other GPU's memory)
-__device__ __forceinline__ void umma_commit_pair_at(uint32_t bar_smem_addr, uint32_t first) {
+// commit of a pair's MMAs onto the barrier at this offset in both of its CTAs (a signal inside one
+// cluster; no load, no other GPU's memory)
+__device__ __forceinline__ void umma_commit_pair_both(uint32_t bar_smem_addr) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(bar_smem_addr), "h"((uint16_t)(3u << first))
+                 ::"r"(bar_smem_addr), "h"((uint16_t)3)
                  : "memory");
 }
 
-template <bool kPair, int kStageKb>   // kStageKb: K blocks of a ring stage
+template <bool kPair>
 __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x, const CUtensorMap* tm_w) {
     extern __shared__ uint8_t mm_smem_raw[];
     uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(mm_smem_raw) + 1023) & ~(uintptr_t)1023);
     constexpr int kXTiles = kPair ? 2 : 1, kSfTiles = 1 + kXTiles;   // scale tiles: weight rows, then 128 rows of x each
     constexpr uint32_t kSfSlotBytes = kSfTiles * kMmSfTile, kSfSlotCols = kSfTiles * 4;
     const uint32_t x_bytes = (uint32_t)a.box * 128u;
-    const uint32_t stage_bytes = (uint32_t)kStageKb * ((uint32_t)kMmWBytes + x_bytes);   // [w]..[x].., tiles of 128-byte rows
+    const uint32_t stage_bytes = (uint32_t)kMmStageKb * ((uint32_t)kMmWBytes + x_bytes);   // [w]..[x].., tiles of 128-byte rows
     uint8_t* sf_tiles = tiles + (size_t)a.n_stages * stage_bytes;
     float* red = reinterpret_cast<float*>(sf_tiles + a.sf_slots * kSfSlotBytes);   // [bt_max][128] partial sums, splits > 1 only
-    MmSmem* S = reinterpret_cast<MmSmem*>(reinterpret_cast<uint8_t*>(red) + (a.splits > 1 ? (size_t)a.bt_max * 512 : 0));
+    const int splits = kPair ? 1 : a.splits;
+    MmSmem* S = reinterpret_cast<MmSmem*>(reinterpret_cast<uint8_t*>(red) + (splits > 1 ? (size_t)a.bt_max * 512 : 0));
     int* start = reinterpret_cast<int*>(S + 1);
     int* before = start + a.experts + 1;  // both [experts + 1]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t ctas = kPair ? 2u : 1u;
-    const uint32_t crank = (kPair || a.splits > 1) ? cluster_ctarank() : 0u;
-    const uint32_t half = kPair ? (crank & 1u) : 0u;          // which CTA of the pair
-    const uint32_t first = kPair ? (crank & ~1u) : crank;     // cluster rank of the pair's leader
+    // a cluster is a pair, or the splits of a tile
+    constexpr uint32_t kCtas = kPair ? 2u : 1u;               // CTAs of a unit that share a tile of accumulators
+    const bool clustered = kPair || splits > 1;
+    const uint32_t crank = clustered ? cluster_ctarank() : 0u;
+    const uint32_t half = kPair ? crank : 0u;                 // which CTA of the pair; the first one leads
     const bool leader = half == 0;
-    const int split = (int)(crank / ctas);
-    const bool clustered = kPair || a.splits > 1;
+    const int split = kPair ? 0 : (int)crank;
     volatile int* abort_flag = &S->abort_flag;
     const uint64_t wait_ns = a.wait_ns;
 
@@ -199,7 +200,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
             tma_prefetch_desc(tm_w);
             tma_prefetch_desc(tm_x);
         }
-        for (int i = lane; i < kMmBarriers; i += 32) mbar_init(&S->full[0] + i, mm_barrier_count(i, ctas, (uint32_t)a.splits));
+        for (int i = lane; i < kMmBarriers; i += 32) mbar_init(&S->full[0] + i, mm_barrier_count(i, kCtas, (uint32_t)splits));
         if (lane == 0) S->abort_flag = 0;
         mbar_fence_init();
         fence_proxy_async_smem();
@@ -258,10 +259,10 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
     if (kPair || (clustered && warp != 0)) cluster_wait();
     const uint32_t tmem_base = warp == 0 ? 0u : *(volatile uint32_t*)&S->tmem_base;
 
-    const int unit = (int)blockIdx.x / (int)(ctas * a.splits), n_units = (int)gridDim.x / (int)(ctas * a.splits);
+    const int cluster = (int)kCtas * splits, unit = (int)blockIdx.x / cluster, n_units = (int)gridDim.x / cluster;
     // K blocks of this split, cut at multiples of four blocks (one scale word holds four)
     const int groups_all = (a.nkb + 3) >> 2;
-    const int g_first = groups_all * split / a.splits, g_last = groups_all * (split + 1) / a.splits;
+    const int g_first = groups_all * split / splits, g_last = groups_all * (split + 1) / splits;
     const int kb_first = g_first * 4, kb_last = min(a.nkb, g_last * 4);
 
     auto wait_bar = [&](uint64_t* bar, uint32_t parity) -> bool {
@@ -269,11 +270,11 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
         else return mbar_wait(bar, parity, wait_ns, abort_flag);
     };
     auto arrive_leader = [&](uint64_t* bar) {
-        if constexpr (kPair) mbar_arrive_cluster(mapa_u32(smem_u32(bar), first));
+        if constexpr (kPair) mbar_arrive_cluster(mapa_u32(smem_u32(bar), 0));
         else mbar_arrive(bar);
     };
     auto drained = [&](uint64_t* bar) {
-        if constexpr (kPair) mbar_arrive_relaxed(mapa_u32(smem_u32(bar), first));
+        if constexpr (kPair) mbar_arrive_relaxed(mapa_u32(smem_u32(bar), 0));
         else mbar_arrive(bar);
     };
     MmTile tl;
@@ -290,16 +291,16 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                 // expert's last row reads the next expert's, and those output columns are not stored
                 const int w_row = (int)((long long)tl.group * a.cols) + tl.w_row + 128 * (int)half;
                 const int x_row = tl.x_row + (kPair ? (int)half * (tl.bt >> 1) : 0);
-                for (int kb = kb_first; kb < kb_last; kb += kStageKb) {
+                for (int kb = kb_first; kb < kb_last; kb += kMmStageKb) {
                     if (!mbar_wait(&S->empty[stage], phase ^ 1, wait_ns, abort_flag)) { dead = true; break; }
                     uint8_t* sw = tiles + (size_t)stage * stage_bytes;
-                    uint8_t* sx = sw + kStageKb * kMmWBytes;
-                    const bool two = kStageKb == 2 && kb + 1 < kb_last;
-                    const uint32_t tx = ctas * ((uint32_t)kMmWBytes + x_bytes) * (two ? 2u : 1u);
+                    uint8_t* sx = sw + kMmStageKb * kMmWBytes;
+                    const bool two = kb + 1 < kb_last;
+                    const uint32_t tx = kCtas * ((uint32_t)kMmWBytes + x_bytes) * (two ? 2u : 1u);
                     uint32_t bar = 0;
                     if constexpr (kPair) {
                         if (leader) mbar_expect_tx(&S->full[stage], tx);
-                        bar = mapa_u32(smem_u32(&S->full[stage]), first);
+                        bar = mapa_u32(smem_u32(&S->full[stage]), 0);
                     } else {
                         mbar_expect_tx(&S->full[stage], tx);
                     }
@@ -352,7 +353,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                 else umma_mxf8(d, wdesc, xdesc, idesc, tsf, tsf + 4, acc);
             };
             auto commit = [&](uint64_t* bar) {
-                if constexpr (kPair) umma_commit_pair_at(smem_u32(bar), first);
+                if constexpr (kPair) umma_commit_pair_both(smem_u32(bar));
                 else umma_commit(bar);
             };
             grid_wait();   // nothing arrives before the loads do: the bounded waits shall not count the kernels before this one
@@ -368,18 +369,18 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                     if (!warp_wait(&S->sf_full[slot], slot_phase)) { dead = true; break; }
                     const uint32_t tsf = tmem_base + (uint32_t)a.sf_col + slot * kSfSlotCols;
 #pragma unroll
-                    for (int i = 0; i < 4; i += kStageKb) {
+                    for (int i = 0; i < 4; i += kMmStageKb) {
                         if (kb0 + i >= kb_last) break;
                         if (!warp_wait(&S->full[stage], phase)) { dead = true; break; }
                         tc_fence_after();
                         const uint64_t wdesc = desc0 + (uint64_t)(stage * desc_step);
-                        const uint64_t xdesc = wdesc + (uint64_t)((kStageKb * kMmWBytes) >> 4);
+                        const uint64_t xdesc = wdesc + (uint64_t)((kMmStageKb * kMmWBytes) >> 4);
                         const uint32_t id0 = idesc0 | ((uint32_t)i << 4) | ((uint32_t)i << 29);        // scale byte i of the group
                         const uint32_t id1 = idesc0 | ((uint32_t)(i + 1) << 4) | ((uint32_t)(i + 1) << 29);
                         if (elected) {
 #pragma unroll
                             for (int k = 0; k < 4; ++k) mma(tacc, wdesc + 2 * k, xdesc + 2 * k, id0, tsf, k ? 1u : acc);
-                            if (kStageKb == 2 && kb0 + i + 1 < kb_last) {
+                            if (kb0 + i + 1 < kb_last) {
 #pragma unroll
                                 for (int k = 0; k < 4; ++k) mma(tacc, wdesc + w_step + 2 * k, xdesc + x_step + 2 * k, id1, tsf, 1u);
                             }
@@ -490,7 +491,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                         tc_fence_after();
 #pragma unroll
                         for (int j = 0; j < kSfTiles; ++j) utccp_32x128b_warpx4_pair(tsf + 4 * j, sfdesc + (j * kMmSfTile >> 4));
-                        umma_commit_pair(mapa_u32(smem_u32(&S->sf_full[slot]), first));
+                        umma_commit_pair(mapa_u32(smem_u32(&S->sf_full[slot]), 0));
                     }
                 } else {
                     tc_fence_after();
@@ -523,7 +524,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
             if (lane == 0) ok = wait_bar(&S->acc_full[buf], use & 1u);
             ok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;
             // every split has added up the previous tile's partials before they are overwritten
-            if (ok && a.splits > 1 && it > 0) ok = mbar_wait_cluster(&S->red_free, (it - 1) & 1u, wait_ns, abort_flag);
+            if (ok && splits > 1 && it > 0) ok = mbar_wait_cluster(&S->red_free, (it - 1) & 1u, wait_ns, abort_flag);
             ok = __all_sync(0xFFFFFFFFu, ok ? 1 : 0) != 0;
             if (!ok) { dead = true; break; }
             tc_fence_after();
@@ -531,7 +532,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
             const uint32_t tacc = tmem_base + buf * (uint32_t)a.bt_max + ((uint32_t)(q * 32) << 16);
             // split K: row r of the tile is added up by split r % splits, into whose shared memory every split writes
             // its partial row, [split][r / splits][128]
-            const int log_splits = __ffs(a.splits) - 1, own_rows = a.bt_max >> log_splits;
+            const int log_splits = __ffs(splits) - 1, own_rows = a.bt_max >> log_splits;
             auto push = [&](int c) {
                 uint32_t v[16];
                 tmem_ld16(tacc + c * 16, v);
@@ -541,14 +542,14 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                 for (int j = 0; j < 16; ++j) {
                     const int r = c * 16 + j;
                     if (r >= tl.valid) break;
-                    const uint32_t owner = (uint32_t)(r & (a.splits - 1)) * ctas + half;
+                    const uint32_t owner = (uint32_t)(r & (splits - 1));
                     st_async_b32(mapa_u32(at + (uint32_t)(r >> log_splits) * 512u, owner), v[j], mapa_u32(bar, owner));
                 }
             };
-            if (a.splits > 1) {
+            if (splits > 1) {
                 // what this CTA will be sent: its rows of the tile, from every split
                 if (warp == kMmFirstEpi && lane == 0)
-                    mbar_expect_tx(&S->red_full, (uint32_t)((tl.valid + a.splits - 1 - split) >> log_splits) * (uint32_t)a.splits * 512u);
+                    mbar_expect_tx(&S->red_full, (uint32_t)((tl.valid + splits - 1 - split) >> log_splits) * (uint32_t)splits * 512u);
 #pragma unroll 1
                 for (int c = part; c < n_chunks; c += 2) push(c);
                 tc_fence_before();
@@ -579,17 +580,17 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                 __syncwarp();
                 if (lane == 0) drained(&S->acc_empty[buf]);
             }
-            if (a.splits > 1) {
+            if (splits > 1) {
                 ok = mbar_wait_cluster(&S->red_full, it & 1u, wait_ns, abort_flag);
                 ok = __all_sync(0xFFFFFFFFu, ok ? 1 : 0) != 0;
                 if (!ok) { dead = true; break; }
                 const bool more = t + n_units < before[a.experts];
                 if (!more) { cluster_arrive(); left = true; }   // nothing of this CTA touches another one's memory from here on
-                const int c0 = tl.w_row + 128 * (int)half + lane * 4;
-                for (int r = split + a.splits * (warp - kMmFirstEpi); r < tl.valid; r += a.splits * kMmEpiWarps) {
+                const int c0 = tl.w_row + lane * 4;
+                for (int r = split + splits * (warp - kMmFirstEpi); r < tl.valid; r += splits * kMmEpiWarps) {
                     const float4* part_row = reinterpret_cast<const float4*>(red + (r >> log_splits) * 128) + lane;
                     float4 sum = part_row[0];
-                    for (int s = 1; s < a.splits; ++s) {
+                    for (int s = 1; s < splits; ++s) {
                         const float4 o = part_row[s * own_rows * 32];
                         sum.x += o.x; sum.y += o.y; sum.z += o.z; sum.w += o.w;
                     }
@@ -606,7 +607,7 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
                 }
                 if (more) {
                     __syncwarp();
-                    if (lane < a.splits) mbar_arrive_cluster(mapa_u32(smem_u32(&S->red_free), (uint32_t)lane * ctas + half));
+                    if (lane < splits) mbar_arrive_cluster(mapa_u32(smem_u32(&S->red_free), (uint32_t)lane));
                 }
             }
         }
@@ -638,10 +639,10 @@ __device__ __forceinline__ void mm_body(const MmArgs& a, const CUtensorMap* tm_x
 // one CTA per tile of 128 weight rows: few rows of x, the weights' stream is all that counts
 __global__ void __launch_bounds__(kMmThreads, 1)
 k_matmul(const MmArgs a, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w) {
-    mm_body<false, kMmStageKb>(a, &tm_x, &tm_w);
+    mm_body<false>(a, &tm_x, &tm_w);
 }
 // a CTA pair per tile of 256 weight rows (2-CTA MMA)
 __global__ void __launch_bounds__(kMmThreads, 1)
 k_matmul_pair(const MmArgs a, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w) {
-    mm_body<true, kMmPairStageKb>(a, &tm_x, &tm_w);
+    mm_body<true>(a, &tm_x, &tm_w);
 }

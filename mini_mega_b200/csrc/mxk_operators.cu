@@ -412,7 +412,7 @@ int mxk_fp8_matmul(const MxkMatmulArgs* p, void* stream) {
     const int sf_tiles = pair ? 3 : 2;
     a.sf_col = 2 * a.bt_max;
     a.sf_slots = std::min(kMmMaxSfSlots, (kMmTmemCols - a.sf_col) / (4 * sf_tiles));
-    const int stage = (pair ? kMmPairStageKb : kMmStageKb) * (kMmWBytes + a.box * 128);
+    const int stage = kMmStageKb * (kMmWBytes + a.box * 128);
     const int fixed = 1024 + a.sf_slots * sf_tiles * kMmSfTile + (a.splits > 1 ? a.bt_max * 512 : 0) + (int)sizeof(MmSmem) + 2 * (a.experts + 1) * 4;
     a.n_stages = std::min(kMmMaxStages, (kMmSmemLimit - fixed) / stage);
     const int smem = fixed + a.n_stages * stage;
@@ -421,7 +421,7 @@ int mxk_fp8_matmul(const MxkMatmulArgs* p, void* stream) {
     if (int rc = byte_map(&tm_w, p->w, experts * cols, depth, p->w_stride, 128)) return rc;
     const auto fn = pair ? k_matmul_pair : k_matmul;
     if (int rc = allow_smem((const void*)fn, pair ? 1 : 2, kMmSmemLimit)) return rc;
-    const int cluster = (pair ? 2 : 1) * a.splits;
+    const int cluster = pair ? 2 : a.splits;   // mm_shape gives pairs no splits
     const int64_t tiles_most = ((p->offsets ? std::min<int64_t>(experts, rows) : 0) + (rows + a.bt_max - 1) / a.bt_max) * a.n_tiles;
     if (tiles_most > (1 << 30)) return fail(MXK_ERR_BAD_ARG, "fp8_matmul: more than 2^30 tiles");
     const dim3 grid((unsigned)(std::min<int64_t>(tiles_most, kSms / cluster) * cluster), 1, 1);
